@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define SUBREG_ABI_VERSION 14
+#define SUBREG_ABI_VERSION 15
 
 #define SUBREG_OK 0
 #define SUBREG_EINVAL (-1)       /* bad argument (null pointer, shape not supported by contract) */
@@ -36,6 +36,9 @@ extern "C" {
 
 #define SUBREG_F32 0  /* exact-f32 MFMA path: the 1e-4 parity gate */
 #define SUBREG_BF16 1 /* bf16 MFMA, fp32 accumulate: the throughput path */
+/* teacher / student operators (subreg_quantize_rows ... subreg_distill_loss) only */
+#define SUBREG_F16 2
+#define SUBREG_I8 3
 
 /* flags of subreg_conv_fwd / subreg_bn_apply */
 #define SUBREG_CONV_LRELU 1     /* nn.LeakyReLU(0.1), models/resnet_language.py:251 */
@@ -442,6 +445,72 @@ int subreg_finetune_step(const subreg_step_desc* d, void* stream);
  * state->epoch (0 when state == NULL); skipped once the stopped loop's last epoch is recorded; mark_done records it */
 int subreg_validate(const float* feat, const long long* labels, const float* weight, const float* bias /* [N] or NULL */, int B, int N, int D,
                     subreg_loop_state* state, int* correct, int set_index, int n_sets_max, int mark_done, void* stream);
+
+/* ---- teacher / student operators: the 8-bit linear head, a row's largest logits, the distillation loss -----------------------
+ * (what the reference's distill/ holds losses for: the answers of a frozen teacher and a student that is trained on them.)
+ * dtype / x_dtype / y_dtype: SUBREG_F32 | SUBREG_BF16 | SUBREG_F16.  Rows are contiguous; `*_stride` is the distance of two rows in
+ * ELEMENTS (0 allowed for inputs: one row seen many times).  Offsets are 64-bit.  Sums and softmax statistics are fp32 or wider.
+ * `ws`: scratch of the size the matching subreg_*_ws_bytes returns, 256-byte aligned, used by this call alone while it runs. */
+
+/* Codes of each row x[r][0..dim): a = max(max_k |x|, 2^-100), scale[r] = a / 127, code = rint(x * (127 / a)) in [-127, 127], where both
+ * quotients and the product are single fp32 operations (the codes are reproducible bit for bit).  codes[r][dim..codes_stride) = 0.
+ * A row that holds a NaN or an infinity gets scale NaN and codes 0: its products are NaN, other rows do not notice. */
+int subreg_quantize_rows(const void* x, long long x_stride, int dtype, int rows, int dim, signed char* codes,
+                         long long codes_stride, float* scale, void* stream);
+
+/* y[r][n] = (float)(sum_k q[r][k] * weight[n][k]) * s[r] * w_scale[n] (+ bias[n]), the sum in 32-bit integers (exact: dim <=
+ * SUBREG_I8_MAX_DIM), one rounding to y_dtype.  x_dtype SUBREG_I8: q = x, s = x_scale.  Otherwise q, s are what subreg_quantize_rows
+ * makes of x, within the call.  y is [rows][out], contiguous.
+ * weight rows: where w_stride and the address are multiples of 16, bytes dim .. round_up(dim, 16) of each row must be readable (their
+ * values do not matter); the same holds for x of SUBREG_I8. */
+#define SUBREG_I8_MAX_DIM 131071
+long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype);
+int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const float* x_scale, const signed char* weight,
+                       long long w_stride, const float* w_scale, const float* bias, void* y, int y_dtype, int rows, int dim,
+                       int out, void* ws, long long ws_bytes, void* stream);
+
+/* The `top` largest logits of each row, largest first: values[rows][top] (dtype), indices[rows][top].  Equal logits (+0 = -0): the lower
+ * index first.  A NaN counts as larger than every number. */
+#define SUBREG_TOP_MAX 256
+int subreg_top_logits(const void* logits, long long stride, int dtype, int rows, int vocab, int top, void* values,
+                      long long* indices, void* stream);
+
+/* Distillation from a teacher's top logits, with the labels' cross entropy in the same pass over the student's logits z:
+ *   entry j of row i is kept if top_indices >= 0 and top_values is not -inf;  p = softmax over the kept entries of top_values / T
+ *   KL_i = sum_j p_j (log p_j - log softmax(z_i / T)[index_j]);   CE_i = -log softmax(z_i)[target_i]
+ *   row i's loss = kd_weight T^2 KL_i + ce_weight CE_i; a row without kept entries has no first term, a row with target ==
+ *   ignore_index (or target == NULL) no second; a row with neither is not read, its loss and its gradient are 0
+ *   reduction: SUBREG_NONE loss[rows]; SUBREG_SUM loss[1]; SUBREG_MEAN loss[1]: each term over the number of ITS rows (no rows: 0)
+ * An index may appear more than once in a row (its shares add).  An index >= vocab, or a target outside [0, vocab) that is not
+ * ignore_index, makes the row's loss and gradient NaN; nothing is read or written out of range.
+ * loss (optional) and dlogits (optional, [rows][vocab] contiguous, dtype of the logits): the gradient times grad_scale[i * grad_scale_stride]
+ * (NULL: 1).  flags: SUBREG_DISTILL_SKIP_UNIT - rows whose grad_scale is exactly 1 are left as they are (they hold this gradient
+ * already); SUBREG_DISTILL_COUNTED - `ws` is the one a call with the same rows, top and reduction has filled. */
+#define SUBREG_NONE 0
+#define SUBREG_SUM 1
+#define SUBREG_MEAN 2
+#define SUBREG_DISTILL_SKIP_UNIT 1
+#define SUBREG_DISTILL_COUNTED 2
+typedef struct {
+    const void* logits;            /* [rows][vocab] */
+    const void* top_values;        /* [rows][top] */
+    const long long* top_indices;  /* [rows][top] */
+    const long long* target;       /* [rows] or NULL */
+    long long logits_stride, values_stride, indices_stride;
+    int dtype, values_dtype;
+    int rows, vocab, top;          /* top <= SUBREG_TOP_MAX */
+    float temperature, kd_weight, ce_weight;
+    long long ignore_index;
+    int reduction, flags;
+    const float* grad_scale;
+    long long grad_scale_stride;   /* 0: one factor for all rows */
+    float* loss;
+    void* dlogits;
+    void* ws;
+    long long ws_bytes;
+} subreg_distill_desc;
+long long subreg_distill_ws_bytes(int rows);
+int subreg_distill_loss(const subreg_distill_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,41 @@
+// Shared pieces of the teacher / student operators (linear_int8.hip, top_logits.hip, distill.hip).
+#pragma once
+#include "subreg_common.h"
+
+namespace subreg {
+
+template <> struct ElemTraits<_Float16> {
+    static constexpr int DT = SUBREG_F16;
+    static __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 from_float(float v) { return (_Float16)v; }
+};
+
+inline bool float_dtype(int dt) { return dt == SUBREG_F32 || dt == SUBREG_BF16 || dt == SUBREG_F16; }
+inline int dtype_bytes(int dt) { return dt == SUBREG_F32 ? 4 : dt == SUBREG_I8 ? 1 : 2; }
+
+// calls F<T>() with the element type of a SUBREG_* float code
+#define SUBREG_FOR_FLOAT(dt, CALL)               \
+    switch (dt) {                                \
+        case SUBREG_F32: { using T = float; CALL; break; }      \
+        case SUBREG_BF16: { using T = __bf16; CALL; break; }    \
+        case SUBREG_F16: { using T = _Float16; CALL; break; }   \
+        default: return SUBREG_EINVAL;           \
+    }
+
+// block reductions over blockDim.x threads (a multiple of 64, <= 1024); result in every thread; `red`: 16 entries of LDS
+template <typename F, typename OP>
+__device__ __forceinline__ F block_reduce(F v, F* red, F neutral, OP op) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    if (nw == 1) return v;
+    __syncthreads();                                  // (a previous reduction's readers are done with `red`)
+    if (lane == 0) red[wid] = v;
+    __syncthreads();
+    v = lane < nw ? red[lane] : neutral;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
+    return __shfl(v, 0);
+}
+
+}  // namespace subreg

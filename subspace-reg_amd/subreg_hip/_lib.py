@@ -13,12 +13,16 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SUBREG_LIB") or os.path.join(_HERE, "libsubreg_hip.so")
 
 F32, BF16 = 0, 1
+F16, I8 = 2, 3                              # teacher / student operators only
 CONV_LRELU, CONV_POOL2, CONV_RAW_STATS = 1, 2, 4
 CONV_KERNEL_GENERAL, CONV_KERNEL_WIDE = 256, 512   # kernel selection of subreg_conv_fwd (Cout % 160 == 0): conv_fwd.hip / conv_wide.hip
 CONV_KERNEL_WIDE_ALT = 1024                        # with _WIDE: the other MFMA shape of conv_wide.hip than its default for the problem
 CONV_KERNEL_WIDE_128, CONV_KERNEL_WIDE_256 = 2048, 4096   # with _WIDE: the 128- / 256-row tiling of conv_wide16_kernel
 FWD_TRAIN = 1
-ABI_VERSION = 14
+ABI_VERSION = 15
+I8_MAX_DIM, TOP_MAX = 131071, 256            # SUBREG_I8_MAX_DIM, SUBREG_TOP_MAX
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+DISTILL_SKIP_UNIT, DISTILL_COUNTED = 1, 2
 MAX_QUERY_SETS = 32                          # SUBREG_MAX_QUERY_SETS
 
 c_void_p, c_int, c_float, c_longlong = C.c_void_p, C.c_int, C.c_float, C.c_longlong
@@ -84,6 +88,15 @@ class StepDesc(C.Structure):
                 ("target_loss", c_float), ("convergence_eps", c_float), ("pull_target", c_void_p),
                 ("adam", c_int), ("beta1", c_float), ("beta2", c_float), ("adam_eps", c_float), ("exp_avg_sq", c_void_p),
                 ("bias", c_void_p), ("bias_momentum_buf", c_void_p), ("bias_exp_avg_sq", c_void_p), ("bias_base", c_void_p)]
+
+
+class DistillDesc(C.Structure):
+    _fields_ = [("logits", c_void_p), ("top_values", c_void_p), ("top_indices", c_void_p), ("target", c_void_p),
+                ("logits_stride", c_longlong), ("values_stride", c_longlong), ("indices_stride", c_longlong),
+                ("dtype", c_int), ("values_dtype", c_int), ("rows", c_int), ("vocab", c_int), ("top", c_int),
+                ("temperature", c_float), ("kd_weight", c_float), ("ce_weight", c_float), ("ignore_index", c_longlong),
+                ("reduction", c_int), ("flags", c_int), ("grad_scale", c_void_p), ("grad_scale_stride", c_longlong),
+                ("loss", c_void_p), ("dlogits", c_void_p), ("ws", c_void_p), ("ws_bytes", c_longlong)]
 
 
 # name -> (restype, argtypes); every symbol include/subreg_hip.h declares
@@ -156,6 +169,12 @@ SIGNATURES = {
     "subreg_loop_state_init": (_I, [_P, _P]),
     "subreg_finetune_step": (_I, [C.POINTER(StepDesc), _P]),
     "subreg_validate": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P]),
+    "subreg_quantize_rows": (_I, [_P, _L, _I, _I, _I, _P, _L, _P, _P]),
+    "subreg_linear_int8_ws_bytes": (_L, [_I, _I, _I, _I]),
+    "subreg_linear_int8": (_I, [_P, _L, _I, _P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P]),
+    "subreg_top_logits": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P]),
+    "subreg_distill_ws_bytes": (_L, [_I]),
+    "subreg_distill_loss": (_I, [C.POINTER(DistillDesc), _P]),
 }
 
 _lib = None

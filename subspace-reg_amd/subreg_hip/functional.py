@@ -3,6 +3,8 @@
 Every op launches a hand-written gfx950 kernel on torch's current stream; torch only owns the
 memory and records the graph.  Reference call sites are named on each class.
 """
+import ctypes as C
+
 import torch
 
 from . import _lib
@@ -195,3 +197,246 @@ class FrobFn(torch.autograd.Function):
         _lib.check(lib.subreg_frob(_lib.ptr(a), _lib.ptr(b), a.numel(), ctx.lmbd, None, _lib.ptr(g), _lib.ptr(ga),
                                    _lib.stream_ptr()), "frob(bwd)")
         return ga, None, None
+
+
+# ---------------------------------------------------------------- teacher / student operators
+# The answers of a frozen teacher (its head in 8 bits, the largest logits of each row) and the loss of a student trained on them
+# (the reference keeps such losses in distill/).  fp32, bf16 and fp16; rows may be strided; any leading dimensions.
+_FLOAT_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_INT_MAX = 2 ** 31 - 1
+
+
+def _float_code(t, name):
+    code = _FLOAT_CODE.get(t.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return code
+
+
+def _on_device(**tensors):
+    """The one device all tensors (None: absent) live on."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError("%s is on %s, the other tensors are on %s" % (name, t.device, dev))
+    if dev.type != "cuda":
+        raise RuntimeError("subreg_hip ops need CUDA (HIP) tensors - there is no CPU fallback (got %s)" % dev)
+    return dev
+
+
+def _rows(t, name):
+    """t as rows: [n, last] with a contiguous last dimension (a copy only where the strides ask for one)."""
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError("%s needs a last dimension of at least one element, got shape %s" % (name, tuple(t.shape)))
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] > _INT_MAX or t.shape[1] > _INT_MAX:
+        raise ValueError("%s: more than 2^31 - 1 rows or columns" % name)
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _launch(dev, fn, what, *args):
+    """fn(*args, stream) on the current stream of `dev`, with `dev` as the current device."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _lib.check(fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), what)
+    return _lib.check(fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def quantize_rows(x):
+    """8-bit codes of each row and their scale: x ~ codes * scale[..., None].
+
+    a = max(max |row|, 2^-100); scale = a / 127; codes = round_half_even(x * (127 / a)), every operation in fp32, so the codes are
+    reproducible bit for bit.  A row with a NaN or an infinity: scale NaN, codes 0.  Returns (codes int8 [..., K], scale fp32 [...]);
+    the codes' rows start at multiples of 16 bytes, the layout linear_int8 reads fastest.  No gradient."""
+    code = _float_code(x, "x")
+    rows = _rows(x.detach(), "x")
+    dev = _on_device(x=x)
+    n, dim = rows.shape
+    pitch = (dim + 15) // 16 * 16
+    codes = torch.empty(n, pitch, dtype=torch.int8, device=dev)
+    scale = torch.empty(n, dtype=torch.float32, device=dev)
+    if n:
+        _launch(dev, _lib.load().subreg_quantize_rows, "quantize_rows", rows.data_ptr(), rows.stride(0), code, n, dim,
+                codes.data_ptr(), pitch, scale.data_ptr())
+    return codes[:, :dim].view(x.shape), scale.view(x.shape[:-1])
+
+
+def _readable16(t):
+    """Whether every row of int8 rows may be read up to the next multiple of 16 columns (which aligned rows are)."""
+    if t.data_ptr() % 16 or t.stride(0) % 16 or t.shape[1] % 16 == 0:
+        return True
+    end = t.storage_offset() + (t.shape[0] - 1) * t.stride(0) + (t.shape[1] + 15) // 16 * 16
+    return end <= t.untyped_storage().nbytes()
+
+
+def linear_int8(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None):
+    """nn.Linear with 8-bit integer operands: y = (codes(x) @ weight^T) * x_scale[..., None] * weight_scale (+ bias).
+
+    weight int8 [N, K], weight_scale fp32 [N] (quantize_rows of the fp32 weight, once), bias fp32 [N] or None.
+    x: float [..., K] - each row ("token") is quantised within the call as quantize_rows does - or int8 codes with x_scale fp32
+    [...].  The integer sums are exact; y is rounded once, to out_dtype (default: x's type, fp32 for codes).
+    For frozen heads: there is no gradient, an x that requires one is refused while autograd records."""
+    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.shape[0] < 1:
+        raise ValueError("weight must be int8 [N, K], got %s %s" % (weight.dtype, tuple(weight.shape)))
+    n, dim = weight.shape
+    if x.dim() < 1 or x.shape[-1] != dim:
+        raise ValueError("x %s does not fit weight %s" % (tuple(x.shape), tuple(weight.shape)))
+    if dim > _lib.I8_MAX_DIM:
+        raise ValueError("K = %d: 32-bit sums are exact up to K = %d" % (dim, _lib.I8_MAX_DIM))
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
+        raise ValueError("weight_scale must be float32 [%d]" % n)
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,)):
+        raise ValueError("bias must be float32 [%d]" % n)
+    if x.dtype == torch.int8:
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1]:
+            raise ValueError("int8 x needs x_scale, float32 %s" % (tuple(x.shape[:-1]),))
+        code = _lib.I8
+    else:
+        if x_scale is not None:
+            raise ValueError("x_scale belongs to int8 x; a float x is quantised here")
+        code = _float_code(x, "x")
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    out_dtype = out_dtype or (torch.float32 if code == _lib.I8 else x.dtype)
+    if out_dtype not in _FLOAT_CODE:
+        raise TypeError("out_dtype must be float32, bfloat16 or float16, got %s" % out_dtype)
+    rows, w = _rows(x, "x"), _rows(weight, "weight")
+    dev = _on_device(x=x, weight=weight, weight_scale=weight_scale, bias=bias, x_scale=x_scale)
+    if not _readable16(w):
+        w = torch.nn.functional.pad(w, (0, -dim % 16))[:, :dim]
+    if code == _lib.I8 and not _readable16(rows):
+        rows = torch.nn.functional.pad(rows, (0, -dim % 16))[:, :dim]
+    m = rows.shape[0]
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    if m:
+        lib = _lib.load()
+        nbytes = lib.subreg_linear_int8_ws_bytes(m, dim, n, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        xs = None if x_scale is None else x_scale.reshape(-1).contiguous()
+        ws_, b_ = weight_scale.contiguous(), None if bias is None else bias.contiguous()
+        _launch(dev, lib.subreg_linear_int8, "linear_int8", rows.data_ptr(), rows.stride(0), code, _ptr(xs), w.data_ptr(), w.stride(0),
+                ws_.data_ptr(), _ptr(b_), y.data_ptr(), _FLOAT_CODE[out_dtype], m, dim, n, ws.data_ptr(), nbytes)
+    return y
+
+
+def top_logits(logits, k):
+    """The k largest logits of each row, largest first, equal ones by the lower index: (values [..., k], indices int64 [..., k]).
+
+    k <= 256.  A NaN counts as larger than every number, so that it shows.  What a teacher's answer is kept as.  No gradient."""
+    code = _float_code(logits, "logits")
+    rows = _rows(logits.detach(), "logits")
+    n, vocab = rows.shape
+    k = int(k)
+    if not 1 <= k <= min(vocab, _lib.TOP_MAX):
+        raise ValueError("k = %d: 1 ... min(%d, %d) are served" % (k, vocab, _lib.TOP_MAX))
+    dev = _on_device(logits=logits)
+    shape = logits.shape[:-1] + (k,)
+    values = torch.empty(shape, dtype=logits.dtype, device=dev)
+    indices = torch.empty(shape, dtype=torch.int64, device=dev)
+    if n:
+        _launch(dev, _lib.load().subreg_top_logits, "top_logits", rows.data_ptr(), rows.stride(0), code, n, vocab, k, values.data_ptr(),
+                indices.data_ptr())
+    return values, indices
+
+
+_REDUCTION = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
+
+
+def _distill_desc(z, tv, ti, target, temperature, kd_weight, ce_weight, ignore_index, reduction, ws):
+    d = _lib.DistillDesc()
+    d.logits, d.top_values, d.top_indices, d.target = z.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(target)
+    d.logits_stride, d.values_stride, d.indices_stride = z.stride(0), tv.stride(0), ti.stride(0)
+    d.dtype, d.values_dtype = _FLOAT_CODE[z.dtype], _FLOAT_CODE[tv.dtype]
+    d.rows, d.vocab, d.top = z.shape[0], z.shape[1], tv.shape[1]
+    d.temperature, d.kd_weight, d.ce_weight, d.ignore_index = temperature, kd_weight, ce_weight, ignore_index
+    d.reduction, d.ws, d.ws_bytes = reduction, ws.data_ptr(), ws.numel()
+    return d
+
+
+class DistillLossFn(torch.autograd.Function):
+    """The loss, and in the same pass over the logits its gradient for an upstream factor of 1 (as CrossEntropyFn does).  The backward
+    hands that gradient on where the factor is 1; elsewhere it is computed again with the factor, in fp32 and rounded once - a
+    gradient scaled after it was rounded would lose what a loss scale is there to keep (fp16)."""
+
+    @staticmethod
+    def forward(ctx, z, tv, ti, target, need_grad, shape, *args):
+        lib, dev = _lib.load(), z.device
+        nbytes = lib.subreg_distill_ws_bytes(z.shape[0])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        d = _distill_desc(z, tv, ti, target, *args, ws)
+        loss = torch.empty(shape, dtype=torch.float32, device=dev)
+        d.loss = loss.data_ptr()
+        if need_grad:
+            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+            d.dlogits = dz.data_ptr()
+            ctx.save_for_backward(z, tv, ti, target)
+            ctx.dz, ctx.ws, ctx.args = dz, ws, args
+        _launch(dev, lib.subreg_distill_loss, "distill_loss", C.byref(d))
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        z, tv, ti, target = ctx.saved_tensors
+        d = _distill_desc(z, tv, ti, target, *ctx.args, ctx.ws)
+        g = g.reshape(-1)
+        d.grad_scale, d.grad_scale_stride = g.data_ptr(), g.stride(0) if g.numel() > 1 else 0
+        d.flags = _lib.DISTILL_COUNTED
+        dz, ctx.dz = ctx.dz, None
+        if dz is None:                               # a second backward over a retained graph: the first took the buffer
+            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        else:
+            d.flags |= _lib.DISTILL_SKIP_UNIT
+        d.dlogits = dz.data_ptr()
+        _launch(z.device, _lib.load().subreg_distill_loss, "distill_loss(bwd)", C.byref(d))
+        return (dz,) + (None,) * (5 + len(ctx.args))
+
+
+def distill_loss(logits, top_values, top_indices, target=None, temperature=1.0, kd_weight=1.0, ce_weight=0.0, ignore_index=-100,
+                 reduction="mean"):
+    """Loss of a student on a teacher's kept logits, with the labels' cross entropy in the same pass.
+
+    logits [..., V] of the student; top_values [..., k], top_indices int64 [..., k] (top_logits of the teacher's; an index < 0 or a
+    value of -inf drops the entry, an index may repeat); target int64 [...] or None.  Per row
+        kd_weight T^2 KL(softmax(top_values / T) || softmax(logits / T)) + ce_weight CE(logits, target)
+    with the teacher's softmax over the row's kept entries.  A row without kept entries has no first term, one whose target is
+    ignore_index no second; a row with neither is not read, its gradient is 0.  reduction "mean": each term over the rows that have it
+    (no such row: 0); "sum"; "none": [...].  Gradient for the logits only, in their type.  An index >= V, or a target outside
+    [0, V), makes its row's loss and gradient NaN."""
+    _float_code(logits, "logits")
+    _float_code(top_values, "top_values")
+    lead = logits.shape[:-1]
+    if top_indices.dtype not in (torch.int64, torch.int32) or (target is not None and target.dtype not in (torch.int64, torch.int32)):
+        raise TypeError("top_indices and target must be int64 or int32")
+    if top_values.shape != top_indices.shape or top_values.shape[:-1] != lead or top_values.dim() != logits.dim():
+        raise ValueError("top_values %s and top_indices %s do not fit logits %s"
+                         % (tuple(top_values.shape), tuple(top_indices.shape), tuple(logits.shape)))
+    if target is not None and target.shape != lead:
+        raise ValueError("target %s does not fit logits %s" % (tuple(target.shape), tuple(logits.shape)))
+    if reduction not in _REDUCTION:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean', got %r" % (reduction,))
+    temperature, kd_weight, ce_weight = float(temperature), float(kd_weight), float(ce_weight)
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be a positive number, got %r" % temperature)
+    if not abs(kd_weight) <= 1e30 or not abs(ce_weight) <= 1e30:
+        raise ValueError("kd_weight and ce_weight must be finite")
+    z, tv, ti = _rows(logits, "logits"), _rows(top_values.detach(), "top_values"), _rows(top_indices, "top_indices").to(torch.int64)
+    if tv.shape[1] > _lib.TOP_MAX:
+        raise ValueError("%d entries a row: at most %d are served" % (tv.shape[1], _lib.TOP_MAX))
+    _on_device(logits=logits, top_values=top_values, top_indices=top_indices, target=target)
+    shape = lead if reduction == "none" else ()
+    if z.shape[0] == 0:
+        empty = z.float().sum(1)
+        return empty.reshape(lead) if reduction == "none" else empty.sum()
+    y = None if target is None or ce_weight == 0.0 else target.reshape(-1).to(torch.int64).contiguous()
+    need = torch.is_grad_enabled() and z.requires_grad
+    return DistillLossFn.apply(z, tv, ti, y, need, shape, temperature, kd_weight, ce_weight, int(ignore_index), _REDUCTION[reduction])

@@ -5,6 +5,8 @@
   train                  train_supervised.py:205-268   one epoch: forward, CE (+ label-pull penalty), meters, backward, SGD step
   validate               eval/util.py:185-232          one pass in eval mode: loss, top-1, top-5
   fit                    train_supervised.py:150-202   epochs, periodic + last checkpoint in the reference's format
+  Teacher                a frozen network whose largest logits a student is trained on (the reference keeps the losses of this in
+                         distill/); `train` / `fit` take one
   GradientSync           replaces nn.DataParallel (:139-140): one process per GPU, every rank takes its share of the batch and
                          back-propagates loss * n_local / n_global; the backbone's flat gradient buffer is SUM-all-reduced
                          stage by stage, overlapped with the backward (RCCL over xGMI), the classifier's at the end
@@ -145,9 +147,54 @@ def _batch_metrics(output, target, counters):
     return loss, 100.0 * c[0] / n, 100.0 * c[1] / n
 
 
-def train(epoch, train_loader, model, criterion, optimizer, opt, lang_puller=None, grad_sync=None, rank=0, world=1, log=print):
+class Teacher:
+    """A frozen network as a teacher: `teacher(images)` -> (values [B, top], indices [B, top]), its `top` largest logits per image.
+
+    int8_head: the classifier's product in 8 bits (functional.linear_int8: codes and scales of the weight are made here, once; the
+    features are quantised per image).  Train a student on it with `train(..., teacher=)` / `fit(..., teacher=)`: the loss is
+    functional.distill_loss with opt.distill_temperature (4), opt.distill_weight (0.5) and opt.distill_ce_weight (0.5).
+    The network is put in eval mode and its weights are taken as they are now."""
+
+    def __init__(self, model, top=10, int8_head=False):
+        self.model = model.eval()
+        self.top = int(top)
+        if not 1 <= self.top <= min(model.num_classes, HF._lib.TOP_MAX):
+            raise ValueError("top = %d of a teacher with %d classes" % (self.top, model.num_classes))
+        self.codes = self.scale = None
+        if int8_head:
+            self.codes, self.scale = HF.quantize_rows(model.classifier.weight.detach())
+
+    @torch.no_grad()
+    def logits(self, images):
+        head = self.model.classifier
+        # (the eager forward: every batch is a new tensor, so the module's replayed and prefetched forwards have nothing to repeat)
+        feat = self.model.hip_backbone().forward(images.float())
+        if self.codes is None:
+            return HF.LinearFn.apply(feat, head.weight, head.bias)
+        return HF.linear_int8(feat, self.codes, self.scale, None if head.bias is None else head.bias.detach())
+
+    def __call__(self, images):
+        return HF.top_logits(self.logits(images), self.top)
+
+
+def _distill(teacher, output, input, target, opt):
+    values, indices = teacher(input)
+    return HF.distill_loss(output, values, indices, target, temperature=getattr(opt, "distill_temperature", 4.0),
+                           kd_weight=getattr(opt, "distill_weight", 0.5), ce_weight=getattr(opt, "distill_ce_weight", 0.5))
+
+
+def train(epoch, train_loader, model, criterion, optimizer, opt, lang_puller=None, grad_sync=None, rank=0, world=1, log=print,
+          teacher=None):
     """train_supervised.py:205-268.  `criterion` is accepted for signature compatibility: CrossEntropyLoss and the accuracy
-    counters are one fused kernel.  Returns (top1.avg, losses.avg)."""
+    counters are one fused kernel.  `teacher` (a Teacher): the loss is the distillation loss on its answers instead of the cross
+    entropy alone.  Returns (top1.avg, losses.avg)."""
+    if teacher is not None:
+        if getattr(opt, "hip_graph", False):
+            raise ValueError("opt.hip_graph captures the step without a teacher: run a distillation eagerly")
+        if teacher.model.num_classes > model.num_classes:
+            raise ValueError("the teacher knows %d classes, the student %d" % (teacher.model.num_classes, model.num_classes))
+        if teacher.model is model:
+            raise ValueError("a network cannot be its own teacher: load the frozen one as a second model")
     model.train()
     batch_time, data_time, losses, top1, top5 = (AverageMeter() for _ in range(5))
     dev = next(model.parameters()).device
@@ -184,7 +231,11 @@ def train(epoch, train_loader, model, criterion, optimizer, opt, lang_puller=Non
             top5.update(acc5, input.size(0))
         else:
             output = model(input)
-            loss, acc1, acc5 = _batch_metrics(output, target, counters)
+            if teacher is None:
+                loss, acc1, acc5 = _batch_metrics(output, target, counters)
+            else:
+                loss = _distill(teacher, output, input, target, opt)
+                _, acc1, acc5 = _batch_metrics(output.detach(), target, counters)
             if getattr(opt, "label_pull", None) is not None and lang_puller is not None:       # :232-236
                 loss = loss + lang_puller.loss1(opt.label_pull, lang_puller(model.classifier.weight), model.classifier.weight)
             losses.update(loss.item(), input.size(0))
@@ -240,9 +291,9 @@ def validate(val_loader, model, criterion, opt, log=print):
     return top1.avg, top5.avg, losses.avg
 
 
-def fit(model, opt, train_loader, val_loader=None, lang_puller=None, rank=0, world=1, group=None, log=print):
+def fit(model, opt, train_loader, val_loader=None, lang_puller=None, rank=0, world=1, group=None, log=print, teacher=None):
     """train_supervised.py:122-202 without the tensorboard logger: optimizer, LR schedule, epochs, periodic and final
-    checkpoints (rank 0 writes).  Returns the per-epoch history."""
+    checkpoints (rank 0 writes).  `teacher`: see `train`.  Returns the per-epoch history."""
     if getattr(opt, "adam", False):                                                              # :128-131
         optimizer = Adam(model.parameters(), lr=opt.learning_rate, weight_decay=0.0005)
     else:                                                                                        # :133-136
@@ -255,7 +306,7 @@ def fit(model, opt, train_loader, val_loader=None, lang_puller=None, rank=0, wor
         model.hip_backbone().grad_stage_hook = sync.stage_ready   # overlap the all-reduce with the backward, stage by stage
     history = []
     try:
-        _fit_epochs(model, opt, train_loader, val_loader, lang_puller, rank, world, log, optimizer, sync, history)
+        _fit_epochs(model, opt, train_loader, val_loader, lang_puller, rank, world, log, optimizer, sync, history, teacher)
     finally:
         if sync is not None:                                    # a backward outside fit() must not start collectives nobody waits on
             model.hip_backbone().grad_stage_hook = None
@@ -266,14 +317,15 @@ def fit(model, opt, train_loader, val_loader=None, lang_puller=None, rank=0, wor
     return history
 
 
-def _fit_epochs(model, opt, train_loader, val_loader, lang_puller, rank, world, log, optimizer, sync, history):
+def _fit_epochs(model, opt, train_loader, val_loader, lang_puller, rank, world, log, optimizer, sync, history,
+                teacher=None):
     for epoch in range(1, opt.epochs + 1):
         set_epoch_lr(epoch, opt, optimizer)
         rec = {"epoch": epoch, "lr": optimizer.param_groups[0]["lr"]}
         if not getattr(opt, "eval_only", False):
             t0 = time.time()
             rec["train_acc"], rec["train_loss"] = train(epoch, train_loader, model, None, optimizer, opt, lang_puller, sync,
-                                                        rank, world, log)
+                                                        rank, world, log, teacher)
             log("epoch {}, total time {:.2f}".format(epoch, time.time() - t0))
         if val_loader is not None:
             rec["test_acc"], rec["test_acc_top5"], rec["test_loss"] = validate(val_loader, model, None, opt, log)
