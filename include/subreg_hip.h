@@ -464,7 +464,7 @@ int subreg_quantize_rows(const void* x, long long x_stride, int dtype, int rows,
  * weight rows: where w_stride and the address are multiples of 16, bytes dim .. round_up(dim, 16) of each row must be readable (their
  * values do not matter); the same holds for x of SUBREG_I8. */
 #define SUBREG_I8_MAX_DIM 131071
-long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype);
+long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype, const signed char* weight, long long w_stride);
 int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const float* x_scale, const signed char* weight,
                        long long w_stride, const float* w_scale, const float* bias, void* y, int y_dtype, int rows, int dim,
                        int out, void* ws, long long ws_bytes, void* stream);

@@ -4,6 +4,8 @@
 //   The sum is exact: |q w| <= 2^14, dim <= 131071 keeps it inside 32 bits, so no rounding depends on the order of K.
 #include "rows_common.h"
 
+#include <type_traits>
+
 namespace subreg {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -42,48 +44,193 @@ __global__ __launch_bounds__(256) void pad_codes_kernel(const signed char* __res
     for (long long k = threadIdx.x; k < codes_stride; k += 256) codes[r * codes_stride + k] = k < dim ? x[r * x_stride + k] : 0;
 }
 
-// 16 bytes of a weight row at any address; bytes at or past `dim` come as zeros and are not read
-__device__ __forceinline__ i32x4 load_codes_tail(const signed char* row, int k, int dim) {
-    i32x4 v = {0, 0, 0, 0};
-    if (k + 16 <= dim) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else {
-        signed char b[16];
-        for (int i = 0; i < 16; ++i) b[i] = k + i < dim ? row[k + i] : 0;
-        __builtin_memcpy(&v, b, 16);
-    }
-    return v;
+// ---------------------------------------------------------------- many rows: tiles through LDS
+// Tile of y: TM = 32 FM rows x TN = 32 FN channels, four waves of (16 FM) x (16 FN), K in stages of 128 bytes, two LDS buffers.
+// v_mfma_i32_16x16x64_i8: an operand lane holds row lane % 16, bytes 16 (lane / 16) .. + 15 of 64; the weights are the first operand, so
+// a result lane holds row m = lane % 16 of x and the channels n = 4 (lane / 16) + i: four neighbours of y, one store.
+// LDS row = 128 bytes = eight 16-byte slots; chunk c of row r sits in slot c ^ (r & 7), so the 16 rows of a fragment read meet every
+// bank group twice (the minimum for 1 KiB).  The permutation is made by the source addresses of the LDS-DMA, inside a 128-byte line.
+// Schedule of a stage (two k-steps): the reads of the second k-step run under the MFMAs of the first; the barrier stands in the MIDDLE
+// of the second k-step's MFMAs, and behind it the DMA of the stage after next and the reads of the next stage's first k-step run under
+// the other half.  A DMA has a whole stage of MFMAs to land.
+// D = C + A B with C and D the same accumulator registers.  As an asm statement because hipcc (ROCm 7.2) gives the builtin's result
+// other registers than its addend and copies between them (376 copies beside the 128 MFMAs of a stage).  The operands come from LDS reads
+// (the compiler waits for those before the statement); before the results are read, mfma_done() lets the last one retire.
+__device__ __forceinline__ void mfma_acc(i32x4& c, const i32x4& a, const i32x4& b) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-// one wave per 16 x 16 tile of y; operands straight from global memory.  A fragment of v_mfma_i32_16x16x64_i8: lane holds row
-// lane % 16, bytes k = 16 (lane / 16) ... + 15; result lane holds column lane % 16, rows 4 (lane / 16) + i.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_int8_kernel(const signed char* __restrict__ q, long long q_stride,
-                                                          const float* __restrict__ s, const signed char* __restrict__ w,
-                                                          long long w_stride, const float* __restrict__ t,
-                                                          const float* __restrict__ bias, T* __restrict__ y, int rows, int dim,
-                                                          int out) {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const long long n0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = (long long)blockIdx.y * 16;
-    if (n0 >= out) return;
-    const signed char* qa = q + min(m0 + l16, (long long)rows - 1) * q_stride;
-    const signed char* wb = w + min(n0 + l16, (long long)out - 1) * w_stride;
-    i32x4 acc = {0, 0, 0, 0};
-    for (int k = g * 16; k - g * 16 < dim; k += 64) {
-        const i32x4 a = *(const i32x4*)(qa + k);
-        const i32x4 b = load_codes_tail(wb, k, dim);
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0);
+template <int FM, int FN> struct TileShape {
+    static constexpr int TM = 32 * FM, TN = 32 * FN, BUF = (TM + TN) * 128, LDS = 2 * BUF, NP = (TM + TN) / 32;
+};
+
+template <int FM, int FN, typename T>
+__global__ __launch_bounds__(256, FM * FN > 16 ? 1 : 2) void linear_int8_tile_kernel(
+    const signed char* __restrict__ q, int q_stride, const float* __restrict__ s, const signed char* __restrict__ w, int w_stride,
+    const float* __restrict__ t, const float* __restrict__ bias, T* __restrict__ y, int rows, int dim, int out) {
+    using S = TileShape<FM, FN>;
+    constexpr int NP = S::NP, NPX = S::TM / 32;                     // 1-KiB DMA pieces (8 rows) of a wave: NPX of x, the rest of w
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    // tiles dealt to the XCDs in contiguous runs, and within a run in blocks of 8 tile rows: neighbours in time share L2 lines
+    int tm, tn;
+    {
+        const int nm = (rows + S::TM - 1) / S::TM, nn = (out + S::TN - 1) / S::TN;
+        const int n = gridDim.x, id = blockIdx.x, q8 = n / 8, r8 = n % 8, xcd = id % 8, slot = id / 8;
+        const int v = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + slot;
+        const int band = v / (8 * nn), in = v - band * 8 * nn, h = min(8, nm - band * 8);
+        tm = band * 8 + in % h;
+        tn = in / h;
     }
-    const long long n = n0 + l16;
-    if (n >= out) return;
-    const float tn = t[n], bn = bias ? bias[n] : 0.f;
+    const int m0 = tm * S::TM, n0 = tn * S::TN;
+
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+    const char* qb = (const char*)q + (long long)m0 * q_stride;
+    const char* wb = (const char*)w + (long long)n0 * w_stride;
+    const int chunk = ((lane & 7) ^ (lane >> 3)) << 4;
+    unsigned off[NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long m = m0 + 4 * g + i;
-        if (m < rows) {
-            float v = (float)acc[i] * s[m] * tn;
-            if (bias) v += bn;
-            y[m * out + n] = ElemTraits<T>::from_float(v);
+    for (int p = 0; p < NP; ++p) {
+        const int r = (wid + 4 * (p < NPX ? p : p - NPX)) * 8 + (lane >> 3);
+        off[p] = p < NPX ? (unsigned)min(r, rows - 1 - m0) * (unsigned)q_stride : (unsigned)min(r, out - 1 - n0) * (unsigned)w_stride;
+    }
+    const int wlast = (dim + 15) / 16 * 16 - 16;                    // last chunk of a weight row that may be read (the codes of x are 0 there)
+    auto dma = [&](int p, int kx, int kw, int buf) {
+        if (p < NPX) dma16(qb, off[p] + (unsigned)kx, lds0 + buf + (wid + 4 * p) * 1024);
+        else dma16(wb, off[p] + (unsigned)kw, lds0 + buf + S::TM * 128 + (wid + 4 * (p - NPX)) * 1024);
+    };
+    auto kx_of = [&](int st) { return st * 128 + chunk; };
+    auto kw_of = [&](int st) { return min(st * 128 + chunk, wlast); };
+
+    const int stages = (dim + 127) / 128;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) dma(p, kx_of(0), kw_of(0), 0);
+    if (stages > 1) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) dma(p, kx_of(1), kw_of(1), S::BUF);
+    }
+
+    const int wm = wid & 1, wn = wid >> 1;
+    const int xa = (wm * FM * 16 + l16) * 128 + ((g ^ (l16 & 7)) << 4);
+    const int wa = (S::TM + wn * FN * 16 + l16) * 128 + ((g ^ (l16 & 7)) << 4);
+    i32x4 acc[FN][FM], fx[2][FM], fw[2][FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+    // read r of a k-step: the first weight fragment, all of x, the other weight fragments
+    auto rd = [&](int r, int set, int buf) {
+        const int x6 = set ? 64 : 0;
+        if (r == 0) fw[set][0] = *(const i32x4*)(smem + buf + (wa ^ x6));
+        else if (r <= FM) fx[set][r - 1] = *(const i32x4*)(smem + buf + (xa ^ x6) + (r - 1) * 2048);
+        else fw[set][r - FM] = *(const i32x4*)(smem + buf + (wa ^ x6) + (r - FM) * 2048);
+    };
+    auto mma = [&](int e, int set) {
+        const int j = e / FM, i = e % FM;
+        mfma_acc(acc[j][i], fw[set][j], fx[set][i]);
+    };
+    auto settle_acc = [&]() {                                       // (every access of acc before this stays before, every one behind it behind)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) asm volatile("" : "+a"(acc[j][i]));
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) asm volatile("" : "+a"(acc[j][i]));
+    };
+    constexpr int NM = FM * FN, NR = FM + FN, HALF = NM / 2;
+    auto stage = [&](int st, int buf, auto next_c, auto dma_c) {
+        constexpr bool NEXT = decltype(next_c)::value, DMA = decltype(dma_c)::value;
+        int rdone = 0;
+#pragma unroll
+        for (int e = 0; e < NM; ++e) {
+            mma(e, 0);
+            if ((e + 1) * NR / NM > rdone) {
+                rd(rdone++, 1, buf);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < HALF; ++e) mma(e, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NEXT) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int kx = kx_of(st + 2), kw = kw_of(st + 2);
+        int rn = 0, dn = 0;
+#pragma unroll
+        for (int e = HALF; e < NM; ++e) {
+            mma(e, 1);
+            if constexpr (NEXT) {
+                if ((e + 1 - HALF) * NR / HALF > rn) {
+                    rd(rn++, 0, buf ^ S::BUF);
+                    if constexpr (NR / HALF > 0) while ((e + 1 - HALF) * NR / HALF > rn) rd(rn++, 0, buf ^ S::BUF);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (DMA) {
+                while ((e + 1 - HALF) * NP / HALF > dn) {
+                    dma(dn++, kx, kw, buf);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    static_assert((S::BUF & (S::BUF - 1)) == 0, "the buffers are switched by an exclusive or");
+    using Yes = std::integral_constant<bool, true>;
+    using No = std::integral_constant<bool, false>;
+    if (stages > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NP) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < NR; ++r) rd(r, 0, 0);
+    settle_acc();                                                    // the zeros are in the accumulators before the first MFMA adds to them
+    int st = 0, buf = 0;
+    for (; st + 2 < stages; ++st, buf ^= S::BUF) stage(st, buf, Yes{}, Yes{});
+    if (st + 1 < stages) {
+        stage(st, buf, Yes{}, No{});
+        buf ^= S::BUF;
+    }
+    stage(st, buf, No{}, No{});
+
+    settle_acc();
+
+    // four neighbours of y per lane and (i, j)
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    const bool whole = n0 + S::TN <= out && (out & 3) == 0;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + (wn * FN + j) * 16 + 4 * g;
+        float tn[4], bn[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int nc = min(n + c, out - 1);
+            tn[c] = t[nc];
+            bn[c] = bias ? bias[nc] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int m = m0 + (wm * FM + i) * 16 + l16;
+            if (m >= rows) continue;
+            const float sm = s[m];
+            T* row = y + (long long)m * out;
+            T v[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float f = (float)acc[j][i][c] * sm * tn[c];
+                v[c] = ElemTraits<T>::from_float(bias ? f + bn[c] : f);
+            }
+            if (whole) {
+                *(T4*)(row + n) = T4{v[0], v[1], v[2], v[3]};
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n + c < out) row[n + c] = v[c];
+            }
         }
     }
 }
@@ -105,10 +252,30 @@ extern "C" int subreg_quantize_rows(const void* x, long long x_stride, int dtype
     return quantize(x, x_stride, dtype, rows, dim, codes, codes_stride, scale, (hipStream_t)stream);
 }
 
-extern "C" long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype) {
-    if (rows <= 0 || dim <= 0 || dim > SUBREG_I8_MAX_DIM || out <= 0 || !(float_dtype(x_dtype) || x_dtype == SUBREG_I8))
+// the weight as the tile kernel reads it: rows at multiples of 16 bytes, 32-bit offsets inside a tile
+static bool weight_direct(const signed char* w, long long w_stride) {
+    return ((size_t)w & 15) == 0 && w_stride % 16 == 0 && w_stride <= (1 << 22);
+}
+
+extern "C" long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype, const signed char* weight, long long w_stride) {
+    if (rows <= 0 || dim <= 0 || dim > SUBREG_I8_MAX_DIM || out <= 0 || w_stride < 0 || !(float_dtype(x_dtype) || x_dtype == SUBREG_I8))
         return SUBREG_EINVAL;
-    return round_up(rows * round_up(dim, I8_PITCH), 256) + round_up(4ll * rows, 256);
+    const long long pitch = round_up(dim, I8_PITCH);
+    return round_up(rows * pitch, 256) + round_up(4ll * rows, 256) + (weight_direct(weight, w_stride) ? 0 : round_up(out * pitch, 256));
+}
+
+template <int FM, int FN, typename T>
+static int launch_tiles(const signed char* q, int pitch, const float* s, const signed char* w, int w_stride, const float* t,
+                        const float* bias, void* y, int rows, int dim, int out, hipStream_t st) {
+    using S = TileShape<FM, FN>;
+    static std::atomic<unsigned long long> ready{0};
+    auto kern = linear_int8_tile_kernel<FM, FN, T>;
+    const int rc = ensure_dynamic_lds((const void*)kern, S::LDS, ready);
+    if (rc) return rc;
+    const long long tiles = (long long)((rows + S::TM - 1) / S::TM) * ((out + S::TN - 1) / S::TN);
+    if (tiles > 0x7fffffff) return SUBREG_EUNSUPPORTED;
+    hipLaunchKernelGGL(kern, (unsigned)tiles, 256, S::LDS, st, q, pitch, s, w, w_stride, t, bias, (T*)y, rows, dim, out);
+    return launch_status();
 }
 
 extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const float* x_scale, const signed char* weight,
@@ -117,7 +284,7 @@ extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype
     SUBREG_CHECK_ARG(x && weight && w_scale && y && ws && rows > 0 && dim > 0 && dim <= SUBREG_I8_MAX_DIM && out > 0);
     SUBREG_CHECK_ARG(x_stride >= 0 && w_stride >= 0 && float_dtype(y_dtype) && (float_dtype(x_dtype) || x_dtype == SUBREG_I8));
     SUBREG_CHECK_ARG((x_dtype == SUBREG_I8) == (x_scale != nullptr) && ((size_t)ws & 255) == 0);
-    SUBREG_CHECK_ARG(ws_bytes >= subreg_linear_int8_ws_bytes(rows, dim, out, x_dtype));
+    SUBREG_CHECK_ARG(ws_bytes >= subreg_linear_int8_ws_bytes(rows, dim, out, x_dtype, weight, w_stride));
     hipStream_t st = (hipStream_t)stream;
     const long long pitch = round_up(dim, I8_PITCH);
     signed char* q = (signed char*)ws;
@@ -129,8 +296,16 @@ extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype
         if (rc) return rc;
     }
     const float* sx = x_dtype == SUBREG_I8 ? x_scale : s;
-    const dim3 grid((out + 63) / 64, (rows + 15) / 16);
-    SUBREG_FOR_FLOAT(y_dtype, hipLaunchKernelGGL(linear_int8_kernel<T>, grid, 256, 0, st, q, pitch, sx, weight, w_stride, w_scale,
-                                                 bias, (T*)y, rows, dim, out))
-    return launch_status();
+    if (!weight_direct(weight, w_stride)) {
+        signed char* wp = (signed char*)s + round_up(4ll * rows, 256);
+        hipLaunchKernelGGL(pad_codes_kernel, out, 256, 0, st, weight, w_stride, dim, wp, pitch);
+        weight = wp;
+        w_stride = pitch;
+    }
+    const bool large = (long long)((rows + 255) / 256) * ((out + 255) / 256) >= 200;
+    SUBREG_FOR_FLOAT(y_dtype, {
+        if (large) return launch_tiles<8, 8, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+        return launch_tiles<4, 4, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+    })
+    return SUBREG_EINVAL;
 }

@@ -14,11 +14,11 @@ inline bool float_dtype(int dt) { return dt == SUBREG_F32 || dt == SUBREG_BF16 |
 inline int dtype_bytes(int dt) { return dt == SUBREG_F32 ? 4 : dt == SUBREG_I8 ? 1 : 2; }
 
 // calls F<T>() with the element type of a SUBREG_* float code
-#define SUBREG_FOR_FLOAT(dt, CALL)               \
+#define SUBREG_FOR_FLOAT(dt, ...)               \
     switch (dt) {                                \
-        case SUBREG_F32: { using T = float; CALL; break; }      \
-        case SUBREG_BF16: { using T = __bf16; CALL; break; }    \
-        case SUBREG_F16: { using T = _Float16; CALL; break; }   \
+        case SUBREG_F32: { using T = float; __VA_ARGS__; break; }      \
+        case SUBREG_BF16: { using T = __bf16; __VA_ARGS__; break; }    \
+        case SUBREG_F16: { using T = _Float16; __VA_ARGS__; break; }   \
         default: return SUBREG_EINVAL;           \
     }
 

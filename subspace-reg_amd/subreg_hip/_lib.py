@@ -170,7 +170,7 @@ SIGNATURES = {
     "subreg_finetune_step": (_I, [C.POINTER(StepDesc), _P]),
     "subreg_validate": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P]),
     "subreg_quantize_rows": (_I, [_P, _L, _I, _I, _I, _P, _L, _P, _P]),
-    "subreg_linear_int8_ws_bytes": (_L, [_I, _I, _I, _I]),
+    "subreg_linear_int8_ws_bytes": (_L, [_I, _I, _I, _I, _P, _L]),
     "subreg_linear_int8": (_I, [_P, _L, _I, _P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P]),
     "subreg_top_logits": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P]),
     "subreg_distill_ws_bytes": (_L, [_I]),

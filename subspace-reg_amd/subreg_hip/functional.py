@@ -319,7 +319,7 @@ def linear_int8(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
     y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
     if m:
         lib = _lib.load()
-        nbytes = lib.subreg_linear_int8_ws_bytes(m, dim, n, code)
+        nbytes = lib.subreg_linear_int8_ws_bytes(m, dim, n, code, w.data_ptr(), w.stride(0))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         xs = None if x_scale is None else x_scale.reshape(-1).contiguous()
         ws_, b_ = weight_scale.contiguous(), None if bias is None else bias.contiguous()

@@ -181,8 +181,8 @@ def test_c_entries_refuse_on_cpu():
     assert lib.subreg_quantize_rows(None, 8, 0, 1, 8, p, 16, p, None) == -1
     assert lib.subreg_quantize_rows(p, 8, 0, 1, 8, p, 7, p, None) == -1
     assert lib.subreg_quantize_rows(p, 8, 3, 1, 8, p, 16, p, None) == -1
-    n = lib.subreg_linear_int8_ws_bytes(4, 100, 7, 0)
-    assert n >= 4 * 100 and lib.subreg_linear_int8_ws_bytes(4, _lib.I8_MAX_DIM + 1, 7, 0) == -1
+    n = lib.subreg_linear_int8_ws_bytes(4, 100, 7, 0, p, 100)
+    assert n >= 4 * 100 and lib.subreg_linear_int8_ws_bytes(4, _lib.I8_MAX_DIM + 1, 7, 0, p, 100) == -1
     args = [p, 100, 0, None, p, 100, p, None, p, 0, 4, 100, 7, p, n, None]
     for at, value in ((0, None), (2, 3), (2, 9), (3, p), (9, 3), (10, 0), (11, 0), (11, _lib.I8_MAX_DIM + 1), (12, 0), (13, None), (13, p + 8),
                       (14, n - 1), (5, -1)):
