@@ -15,26 +15,74 @@ constexpr float I8_FLOOR = 0x1p-100f;    // smallest row maximum: 127 / max stay
 
 static inline long long round_up(long long a, long long b) { return (a + b - 1) / b * b; }
 
-// one block per row: maximum of the magnitudes as integers (a NaN's bits are above infinity's, so both are seen), then the codes
-template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, long long x_stride, int dim,
+// scale and 1 / step of a row whose largest magnitude has the bits `top` (as integers a NaN's bits are above infinity's: both are seen)
+__device__ __forceinline__ float row_inverse(unsigned top, float* scale) {
+    const bool bad = top >= 0x7f800000u;
+    const float amax = fmaxf(__uint_as_float(top), I8_FLOOR);
+    *scale = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(amax, 127.f);
+    return bad ? 0.f : __fdiv_rn(127.f, amax);
+}
+// |x inv| < 127.5 by the choice of inv; in a bad row inv = 0, and the conversion of 0 x infinity = NaN is 0 too
+__device__ __forceinline__ int code_of(float x, float inv) { return __float2int_rn(x * inv); }
+
+// NT threads (a wave or a block of 256) per row, the row in registers: one read of x, 16 bytes a load, codes of a load in one store
+// (loads that overlap at the row's end write the same codes twice).  Bound by memory.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, long long x_stride, int rows, int dim,
                                                             signed char* __restrict__ codes, long long codes_stride,
                                                             float* __restrict__ scale) {
+    constexpr int N = RowVec<T>::N;
+    __shared__ unsigned red[16];
+    const int lane = threadIdx.x % NT;
+    const long long r = (long long)blockIdx.x * (256 / NT) + threadIdx.x / NT;
+    if (r >= rows) return;                            // (whole waves; a block of one row never)
+    const T* row = x + r * x_stride;
+    RowVec<T> v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i].load(row, RowVec<T>::at(i * NT + lane, dim));
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(v[i].get(e)) & 0x7fffffffu);
+    if constexpr (NT == 64) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    } else {
+        top = block_reduce(top, red, 0u, [](unsigned a, unsigned b) { return max(a, b); });
+    }
+    float sc;
+    const float inv = row_inverse(top, &sc);
+    if (lane == 0) scale[r] = sc;
+    signed char* out = codes + r * codes_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = i * NT + lane;
+        signed char q[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[e] = (signed char)code_of(v[i].get(e), inv);
+        if (c * N < dim) __builtin_memcpy(out + RowVec<T>::at(c, dim), q, N);
+    }
+    for (long long k = dim + lane; k < codes_stride; k += NT) out[k] = 0;
+}
+
+// rows shorter than a load, or too long for registers (two reads)
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_any_rows_kernel(const T* __restrict__ x, long long x_stride, int dim,
+                                                                 signed char* __restrict__ codes, long long codes_stride,
+                                                                 float* __restrict__ scale) {
     __shared__ unsigned red[16];
     const long long r = blockIdx.x;
     const T* row = x + r * x_stride;
     unsigned top = 0;
     for (int k = threadIdx.x; k < dim; k += 256) top = max(top, __float_as_uint(ElemTraits<T>::to_float(row[k])) & 0x7fffffffu);
     top = block_reduce(top, red, 0u, [](unsigned a, unsigned b) { return max(a, b); });
-    const bool bad = top >= 0x7f800000u;
-    const float amax = fmaxf(__uint_as_float(top), I8_FLOOR);
-    const float inv = bad ? 0.f : __fdiv_rn(127.f, amax);
-    if (threadIdx.x == 0) scale[r] = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(amax, 127.f);
+    float sc;
+    const float inv = row_inverse(top, &sc);
+    if (threadIdx.x == 0) scale[r] = sc;
     signed char* out = codes + r * codes_stride;
-    for (long long k = threadIdx.x; k < codes_stride; k += 256) {
-        const float v = k < dim && !bad ? rintf(ElemTraits<T>::to_float(row[k]) * inv) : 0.f;
-        out[k] = (signed char)(int)fminf(fmaxf(v, -127.f), 127.f);
-    }
+    for (long long k = threadIdx.x; k < codes_stride; k += 256)
+        out[k] = k < dim ? (signed char)code_of(ElemTraits<T>::to_float(row[k]), inv) : 0;
 }
 
 // x given as codes: rows copied to the padded pitch
@@ -74,16 +122,16 @@ __global__ __launch_bounds__(256, FM * FN > 16 ? 1 : 2) void linear_int8_tile_ke
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     // tiles dealt to the XCDs in contiguous runs, and within a run in blocks of 8 tile rows: neighbours in time share L2 lines
-    int tm, tn;
+    int tile_m, tile_n;
     {
         const int nm = (rows + S::TM - 1) / S::TM, nn = (out + S::TN - 1) / S::TN;
         const int n = gridDim.x, id = blockIdx.x, q8 = n / 8, r8 = n % 8, xcd = id % 8, slot = id / 8;
         const int v = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + slot;
         const int band = v / (8 * nn), in = v - band * 8 * nn, h = min(8, nm - band * 8);
-        tm = band * 8 + in % h;
-        tn = in / h;
+        tile_m = band * 8 + in % h;
+        tile_n = in / h;
     }
-    const int m0 = tm * S::TM, n0 = tn * S::TN;
+    const int m0 = tile_m * S::TM, n0 = tile_n * S::TN;
 
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
     const char* qb = (const char*)q + (long long)m0 * q_stride;
@@ -199,46 +247,63 @@ __global__ __launch_bounds__(256, FM * FN > 16 ? 1 : 2) void linear_int8_tile_ke
 
     settle_acc();
 
-    // four neighbours of y per lane and (i, j)
+    // four neighbours of y per lane and (i, j); the scales are in registers before the first store (a load behind a store would wait)
     typedef __attribute__((ext_vector_type(4))) T T4;
-    const bool whole = n0 + S::TN <= out && (out & 3) == 0;
+    const bool whole = m0 + S::TM <= rows && n0 + S::TN <= out && (out & 3) == 0;
+    float sm[FM];
+    f32x4 tn[FN], bn[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sm[i] = s[min(m0 + (wm * FM + i) * 16 + l16, rows - 1)];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int n = n0 + (wn * FN + j) * 16 + 4 * g;
-        float tn[4], bn[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int nc = min(n + c, out - 1);
-            tn[c] = t[nc];
-            bn[c] = bias ? bias[nc] : 0.f;
-        }
+        for (int c = 0; c < 4; ++c) tn[j][c] = t[min(n + c, out - 1)];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const int m = m0 + (wm * FM + i) * 16 + l16;
-            if (m >= rows) continue;
-            const float sm = s[m];
-            T* row = y + (long long)m * out;
+        for (int c = 0; c < 4; ++c) bn[j][c] = bias ? bias[min(n + c, out - 1)] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = m0 + (wm * FM + i) * 16 + l16;
+        T* row = y + (long long)m * out + n0 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
             T v[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float f = (float)acc[j][i][c] * sm * tn[c];
-                v[c] = ElemTraits<T>::from_float(bias ? f + bn[c] : f);
-            }
+            for (int c = 0; c < 4; ++c) v[c] = ElemTraits<T>::from_float((float)acc[j][i][c] * sm[i] * tn[j][c] + bn[j][c]);
+            const int nl = (wn * FN + j) * 16;
             if (whole) {
-                *(T4*)(row + n) = T4{v[0], v[1], v[2], v[3]};
-            } else {
+                *(T4*)(row + nl) = T4{v[0], v[1], v[2], v[3]};
+            } else if (m < rows) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (n + c < out) row[n + c] = v[c];
+                    if (n0 + nl + 4 * g + c < out) row[nl + c] = v[c];
             }
         }
     }
 }
 
+template <typename T>
+static void launch_quantize(const T* x, long long x_stride, int rows, int dim, signed char* codes, long long codes_stride, float* scale,
+                            hipStream_t s) {
+    constexpr int N = RowVec<T>::N;
+    const int loads = (dim + N - 1) / N, four = (int)(((long long)rows + 3) / 4);
+#define SUBREG_QUANT(NT, NV, GRID) \
+    hipLaunchKernelGGL((quantize_rows_kernel<T, NT, NV>), GRID, 256, 0, s, x, x_stride, rows, dim, codes, codes_stride, scale)
+    if (dim < N || loads > 256 * 16)
+        hipLaunchKernelGGL(quantize_any_rows_kernel<T>, rows, 256, 0, s, x, x_stride, dim, codes, codes_stride, scale);
+    else if (loads <= 64 * 2) SUBREG_QUANT(64, 2, four);
+    else if (loads <= 64 * 4) SUBREG_QUANT(64, 4, four);
+    else if (loads <= 64 * 8) SUBREG_QUANT(64, 8, four);
+    else if (loads <= 256 * 4) SUBREG_QUANT(256, 4, rows);
+    else if (loads <= 256 * 8) SUBREG_QUANT(256, 8, rows);
+    else SUBREG_QUANT(256, 16, rows);
+#undef SUBREG_QUANT
+}
+
 static int quantize(const void* x, long long x_stride, int dtype, int rows, int dim, signed char* codes, long long codes_stride,
                     float* scale, hipStream_t s) {
-    SUBREG_FOR_FLOAT(dtype, hipLaunchKernelGGL(quantize_rows_kernel<T>, rows, 256, 0, s, (const T*)x, x_stride, dim, codes,
-                                               codes_stride, scale))
+    SUBREG_FOR_FLOAT(dtype, launch_quantize<T>((const T*)x, x_stride, rows, dim, codes, codes_stride, scale, s))
     return launch_status();
 }
 

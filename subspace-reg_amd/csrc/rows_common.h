@@ -38,4 +38,19 @@ __device__ __forceinline__ F block_reduce(F v, F* red, F neutral, OP op) {
     return __shfl(v, 0);
 }
 
+// 16 bytes of a row of n >= N elements, N to a load, without a branch (a load inside a divergent branch is waited for inside it, one
+// after the other).  Load c covers the elements c N ... - or, where that passes the row's end, the row's last N: its first `skip`
+// elements then belong to the load before it (skip >= N: all of them do).  Any alignment of the row: the hardware takes vector
+// accesses at element addresses.
+template <typename T> struct RowVec {
+    static constexpr int N = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(N))) T V;
+    V v;
+    static __device__ __forceinline__ int at(int c, int n) { return min(c * N, n - N); }
+    static __device__ __forceinline__ int skip(int c, int n) { return max(c * N - (n - N), 0); }
+    __device__ __forceinline__ void load(const T* row, int at) { __builtin_memcpy(&v, row + at, 16); }
+    __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy(row + at, &v, 16); }
+    __device__ __forceinline__ float get(int e) const { return ElemTraits<T>::to_float(v[e]); }
+};
+
 }  // namespace subreg
