@@ -449,7 +449,7 @@ int subreg_validate(const float* feat, const long long* labels, const float* wei
 /* ---- teacher / student operators: the 8-bit linear head, a row's largest logits, the distillation loss -----------------------
  * (what the reference's distill/ holds losses for: the answers of a frozen teacher and a student that is trained on them.)
  * dtype / x_dtype / y_dtype: SUBREG_F32 | SUBREG_BF16 | SUBREG_F16.  Rows are contiguous; `*_stride` is the distance of two rows in
- * ELEMENTS (0 allowed for inputs: one row seen many times).  Offsets are 64-bit.  Sums and softmax statistics are fp32 or wider.
+ * ELEMENTS (0 allowed for inputs: one row seen many times).  Up to 2^30 columns; offsets are 64-bit.  Sums and softmax statistics are fp32 or wider.
  * `ws`: scratch of the size the matching subreg_*_ws_bytes returns, 256-byte aligned, used by this call alone while it runs. */
 
 /* Codes of each row x[r][0..dim): a = max(max_k |x|, 2^-100), scale[r] = a / 127, code = rint(x * (127 / a)) in [-127, 127], where both
@@ -472,8 +472,9 @@ int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const flo
 /* The `top` largest logits of each row, largest first: values[rows][top] (dtype), indices[rows][top].  Equal logits (+0 = -0): the lower
  * index first.  A NaN counts as larger than every number. */
 #define SUBREG_TOP_MAX 256
+long long subreg_top_logits_ws_bytes(int rows, int vocab, int top);   /* 0: no scratch needed, ws may be NULL */
 int subreg_top_logits(const void* logits, long long stride, int dtype, int rows, int vocab, int top, void* values,
-                      long long* indices, void* stream);
+                      long long* indices, void* ws, long long ws_bytes, void* stream);
 
 /* Distillation from a teacher's top logits, with the labels' cross entropy in the same pass over the student's logits z:
  *   entry j of row i is kept if top_indices >= 0 and top_values is not -inf;  p = softmax over the kept entries of top_values / T

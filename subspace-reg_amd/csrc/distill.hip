@@ -229,7 +229,7 @@ extern "C" long long subreg_distill_ws_bytes(int rows) {
 
 extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     SUBREG_CHECK_ARG(d && d->logits && d->top_values && d->top_indices && (d->loss || d->dlogits));
-    SUBREG_CHECK_ARG(d->rows > 0 && d->vocab > 0 && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
+    SUBREG_CHECK_ARG(d->rows > 0 && d->vocab > 0 && d->vocab <= MAX_COLUMNS && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
     SUBREG_CHECK_ARG(d->logits_stride >= 0 && d->values_stride >= 0 && d->indices_stride >= 0 && d->grad_scale_stride >= 0);
     SUBREG_CHECK_ARG(float_dtype(d->dtype) && float_dtype(d->values_dtype) && d->temperature > 0.f && d->temperature <= 3.0e38f);
     SUBREG_CHECK_ARG(d->reduction >= SUBREG_NONE && d->reduction <= SUBREG_MEAN);

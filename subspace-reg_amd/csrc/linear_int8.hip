@@ -313,7 +313,7 @@ using namespace subreg;
 
 extern "C" int subreg_quantize_rows(const void* x, long long x_stride, int dtype, int rows, int dim, signed char* codes,
                                     long long codes_stride, float* scale, void* stream) {
-    SUBREG_CHECK_ARG(x && codes && scale && rows > 0 && dim > 0 && x_stride >= 0 && codes_stride >= dim && float_dtype(dtype));
+    SUBREG_CHECK_ARG(x && codes && scale && rows > 0 && dim > 0 && dim <= MAX_COLUMNS && x_stride >= 0 && codes_stride >= dim && float_dtype(dtype));
     return quantize(x, x_stride, dtype, rows, dim, codes, codes_stride, scale, (hipStream_t)stream);
 }
 

@@ -10,6 +10,8 @@ template <> struct ElemTraits<_Float16> {
     static __device__ __forceinline__ _Float16 from_float(float v) { return (_Float16)v; }
 };
 
+constexpr int MAX_COLUMNS = 1 << 30;      // of a row: column arithmetic stays inside 32 bits
+
 inline bool float_dtype(int dt) { return dt == SUBREG_F32 || dt == SUBREG_BF16 || dt == SUBREG_F16; }
 inline int dtype_bytes(int dt) { return dt == SUBREG_F32 ? 4 : dt == SUBREG_I8 ? 1 : 2; }
 
@@ -45,12 +47,16 @@ __device__ __forceinline__ F block_reduce(F v, F* red, F neutral, OP op) {
 template <typename T> struct RowVec {
     static constexpr int N = 16 / sizeof(T);
     typedef __attribute__((ext_vector_type(N))) T V;
-    V v;
+    typedef __attribute__((ext_vector_type(4))) unsigned U;
+    U raw;
     static __device__ __forceinline__ int at(int c, int n) { return min(c * N, n - N); }
     static __device__ __forceinline__ int skip(int c, int n) { return max(c * N - (n - N), 0); }
-    __device__ __forceinline__ void load(const T* row, int at) { __builtin_memcpy(&v, row + at, 16); }
-    __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy(row + at, &v, 16); }
-    __device__ __forceinline__ float get(int e) const { return ElemTraits<T>::to_float(v[e]); }
+    __device__ __forceinline__ void load(const T* row, int at) { __builtin_memcpy(&raw, row + at, 16); }
+    __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy(row + at, &raw, 16); }
+    __device__ __forceinline__ T elem(int e) const { return __builtin_bit_cast(V, raw)[e]; }
+    __device__ __forceinline__ float get(int e) const { return ElemTraits<T>::to_float(elem(e)); }
+    // between two uses of a held row: what the first use unpacked is unpacked again (kept, it would take twice the registers)
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(raw)); }
 };
 
 }  // namespace subreg

@@ -203,7 +203,6 @@ class FrobFn(torch.autograd.Function):
 # The answers of a frozen teacher (its head in 8 bits, the largest logits of each row) and the loss of a student trained on them
 # (the reference keeps such losses in distill/).  fp32, bf16 and fp16; rows may be strided; any leading dimensions.
 _FLOAT_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
-_INT_MAX = 2 ** 31 - 1
 
 
 def _float_code(t, name):
@@ -234,8 +233,8 @@ def _rows(t, name):
         raise ValueError("%s needs a last dimension of at least one element, got shape %s" % (name, tuple(t.shape)))
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] > _INT_MAX or t.shape[1] > _INT_MAX:
-        raise ValueError("%s: more than 2^31 - 1 rows or columns" % name)
+    if t.shape[0] > 2 ** 31 - 1 or t.shape[1] > 2 ** 30:
+        raise ValueError("%s: more than 2^31 - 1 rows or 2^30 columns" % name)
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -343,8 +342,11 @@ def top_logits(logits, k):
     values = torch.empty(shape, dtype=logits.dtype, device=dev)
     indices = torch.empty(shape, dtype=torch.int64, device=dev)
     if n:
-        _launch(dev, _lib.load().subreg_top_logits, "top_logits", rows.data_ptr(), rows.stride(0), code, n, vocab, k, values.data_ptr(),
-                indices.data_ptr())
+        lib = _lib.load()
+        nbytes = lib.subreg_top_logits_ws_bytes(n, vocab, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _launch(dev, lib.subreg_top_logits, "top_logits", rows.data_ptr(), rows.stride(0), code, n, vocab, k, values.data_ptr(),
+                indices.data_ptr(), _ptr(ws), nbytes)
     return values, indices
 
 

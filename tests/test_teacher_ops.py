@@ -189,8 +189,12 @@ def test_c_entries_refuse_on_cpu():
         bad = list(args)
         bad[at] = value
         assert lib.subreg_linear_int8(*bad) == -1, at
-    for bad in ((None, 8, 0, 1, 8, 1, p, p, None), (p, 8, 0, 1, 8, 9, p, p, None), (p, 300, 0, 1, 300, 257, p, p, None),
-                (p, 8, 3, 1, 8, 1, p, p, None), (p, -1, 0, 1, 8, 1, p, p, None), (p, 8, 0, 0, 8, 1, p, p, None)):
+    assert lib.subreg_top_logits_ws_bytes(64, 1000, 5) == 0 and lib.subreg_top_logits_ws_bytes(1, 8, 9) == -1
+    n = lib.subreg_top_logits_ws_bytes(1, 100000, 5)
+    for bad in ((None, 8, 0, 1, 8, 1, p, p, None, 0, None), (p, 8, 0, 1, 8, 9, p, p, None, 0, None), (p, 300, 0, 1, 300, 257, p, p, None, 0, None),
+                (p, 8, 3, 1, 8, 1, p, p, None, 0, None), (p, -1, 0, 1, 8, 1, p, p, None, 0, None), (p, 8, 0, 0, 8, 1, p, p, None, 0, None),
+                (p, 8, 0, 1, 100000, 5, p, p, None, n, None), (p, 8, 0, 1, 100000, 5, p, p, p + 8, n, None),
+                (p, 8, 0, 1, 100000, 5, p, p, p, n - 1, None)):
         assert lib.subreg_top_logits(*bad) == -1
     assert lib.subreg_distill_ws_bytes(0) == -1
 
@@ -325,7 +329,7 @@ def check_top(z, k):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (3, 2, 2), (64, 351, 5), (5, 60, 60), (2, 256, 256), (7, 1000, 17), (3, 1025, 256),
-                                          (2, 5003, 64), (9, 32000, 32), (1, 131072, 128), (2, 140001, 256), (1, 300007, 33)])
+                                          (2, 5003, 64), (9, 32000, 32), (1, 16384, 256), (1, 16385, 1), (3, 131071, 256), (60, 20011, 40), (300, 33333, 50), (1, 131072, 128), (2, 140001, 256), (1, 300007, 33)])
 def test_top_logits(rows, vocab, k, dtype):
     check_top(rnd((rows, vocab), vocab + k, dtype, 2.5), k)
 
