@@ -470,11 +470,10 @@ int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const flo
                        int out, void* ws, long long ws_bytes, void* stream);
 
 /* The `top` largest logits of each row, largest first: values[rows][top] (dtype), indices[rows][top].  Equal logits (+0 = -0): the lower
- * index first.  A NaN counts as larger than every number. */
+ * index first.  A NaN counts as larger than every number.  (A zero is returned as +0, a NaN as one NaN.) */
 #define SUBREG_TOP_MAX 256
-long long subreg_top_logits_ws_bytes(int rows, int vocab, int top);   /* 0: no scratch needed, ws may be NULL */
 int subreg_top_logits(const void* logits, long long stride, int dtype, int rows, int vocab, int top, void* values,
-                      long long* indices, void* ws, long long ws_bytes, void* stream);
+                      long long* indices, void* stream);
 
 /* Distillation from a teacher's top logits, with the labels' cross entropy in the same pass over the student's logits z:
  *   entry j of row i is kept if top_indices >= 0 and top_values is not -inf;  p = softmax over the kept entries of top_values / T

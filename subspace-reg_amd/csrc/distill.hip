@@ -2,13 +2,19 @@
 //   p = softmax over a row's kept entries of t / T;  e_v = exp((z_v - m) / T), S = sum_v e_v;  likewise at T = 1 for the labels
 //   KL = sum_j p_j (log p_j - (z_{i_j} - m) / T + log S);        CE = log S_1 - (z_y - m)
 //   d(a T^2 KL)/dz_v = a T (e_v / S - sum_{j: i_j = v} p_j);     d(b CE)/dz_v = b (e1_v / S_1 - [v = y])
-// Every row needs its maximum and two sums before its first gradient is known, so a row is read, reduced and written by one block.
+// Every row needs its maximum and two sums before its first gradient is known, so a row is read, reduced and written by one block, and
+// held in its registers in between: each logit is read once and each gradient written once.
+// All exponents are x_v = z_v c - m c (c = log2(e) / T, one fused operation, m c rounded once and common to the row): its error is one
+// rounding of x_v, and the common one cancels in every quotient.  Where T is a power of two, e1 = e^T by squarings (one instruction
+// each, where a second exponential is five).
 #include "rows_common.h"
+
+#include <type_traits>
 
 namespace subreg {
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int COUNT_ROWS = 64;           // rows whose entries one block of the counting kernel looks at
+constexpr int COUNT_BLOCKS = 256;        // at most, of the counting kernel
 
 struct DistillArgs {
     const void* z;
@@ -16,7 +22,7 @@ struct DistillArgs {
     const long long* ti;
     const long long* target;
     long long z_stride, tv_stride, ti_stride, ignore;
-    int rows, vocab, top, reduction, flags, same_t, count_blocks;
+    int rows, vocab, top, reduction, flags, count_blocks, count_rows, squarings;
     float c_t, inv_t, kd, ce, temp;      // c_t = log2(e) / T
     const float* gs;
     long long gs_stride;
@@ -41,8 +47,8 @@ __global__ __launch_bounds__(256) void distill_count_kernel(DistillArgs a) {
     __shared__ int red[16];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     int kd = 0, ce = 0;
-    for (int i = wid; i < COUNT_ROWS; i += 4) {
-        const long long r = (long long)blockIdx.x * COUNT_ROWS + i;
+    for (int i = wid; i < a.count_rows; i += 4) {
+        const long long r = (long long)blockIdx.x * a.count_rows + i;
         if (r >= a.rows) break;
         bool any = false;
         for (int j = lane; j < a.top; j += 64) {
@@ -86,16 +92,17 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(DistillArgs a) {
     if (threadIdx.x == 0) a.loss[0] = (float)((double)a.kd * a.temp * a.temp * kd + (double)a.ce * ce);
 }
 
-template <typename T, typename TV>
-__global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
+// any row: shorter than a load, longer than the registers hold, or with a maximum so large that m c is not a number to subtract
+// (logits of the type's lowest value, infinities).  NT threads of one row; reads it three times, from the caches after the first.
+template <typename T, typename TV, int NT>
+__device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long r) {
     __shared__ float red[16];
     __shared__ int redi[16];
     __shared__ float s_p[SUBREG_TOP_MAX + 1];
     __shared__ int s_i[SUBREG_TOP_MAX + 1];          // vocabulary entry, -1: none; the label is entry `top`
-    const long long r = blockIdx.x;
     const int tid = threadIdx.x;
     const float g = a.gs ? a.gs[r * a.gs_stride] : 1.f;
-    if ((a.flags & SUBREG_DISTILL_SKIP_UNIT) && g == 1.f) return;
+    __syncthreads();
     const T* z = (const T*)a.z + r * a.z_stride;
     T* dz = a.dz ? (T*)a.dz + r * a.vocab : nullptr;
     auto add = [](float p, float q) { return p + q; };
@@ -105,6 +112,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
     // the teacher's share
     float tv = -INFINITY;
     long long ti = -1;
+    static_assert(NT >= SUBREG_TOP_MAX, "one entry a thread");
     const bool kept = tid < a.top && entry_kept<TV>(a, r, tid, tv, ti);
     const bool wild = kept && ti >= a.vocab;
     const int state = block_reduce((kept ? 1 : 0) + (wild ? 1 << 16 : 0), redi, 0, addi);
@@ -121,7 +129,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
     float cnt_kd = 1.f, cnt_ce = 1.f;
     if (a.reduction == SUBREG_MEAN && dz) {
         int n_kd = 0, n_ce = 0;
-        for (int b = tid; b < a.count_blocks; b += 256) {
+        for (int b = tid; b < a.count_blocks; b += NT) {
             n_kd += a.counts[2 * b];
             n_ce += a.counts[2 * b + 1];
         }
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
     float* out = a.reduction == SUBREG_NONE ? a.loss : nullptr;
     if (!kd_on && !ce_on) {
         if (dz)
-            for (int v = tid; v < a.vocab; v += 256) dz[v] = ElemTraits<T>::from_float(0.f);
+            for (int v = tid; v < a.vocab; v += NT) dz[v] = ElemTraits<T>::from_float(0.f);
         if (tid == 0 && a.loss) {
             if (out) out[r] = 0.f;
             else { a.row_kd[r] = 0.f; a.row_ce[r] = 0.f; }
@@ -153,16 +161,16 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
 
     // the student's softmax
     float m = -INFINITY;
-    for (int v = tid; v < a.vocab; v += 256) m = fmaxf(m, ElemTraits<T>::to_float(z[v]));
+    for (int v = tid; v < a.vocab; v += NT) m = fmaxf(m, ElemTraits<T>::to_float(z[v]));
     m = block_reduce(m, red, -INFINITY, mx);
     float se = 0.f, s1 = 0.f;
-    for (int v = tid; v < a.vocab; v += 256) {
+    for (int v = tid; v < a.vocab; v += NT) {
         const float d = ElemTraits<T>::to_float(z[v]) - m;
         se += exp2_fast(d * a.c_t);
-        if (ce_on && !a.same_t) s1 += exp2_fast(d * LOG2E);
+        if (ce_on && !(a.squarings == 0)) s1 += exp2_fast(d * LOG2E);
     }
     se = block_reduce(se, red, 0.f, add);
-    s1 = a.same_t ? se : block_reduce(s1, red, 0.f, add);
+    s1 = (a.squarings == 0) ? se : block_reduce(s1, red, 0.f, add);
 
     if (a.loss) {
         float term = 0.f;
@@ -182,15 +190,15 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
     const float akd = ckd / se, ace = cce / s1;
     auto grad = [&](float zv, float pv, float hot) {
         const float d = zv - m;
-        const float et = exp2_fast(d * a.c_t), e1 = a.same_t ? et : exp2_fast(d * LOG2E);
+        const float et = exp2_fast(d * a.c_t), e1 = (a.squarings == 0) ? et : exp2_fast(d * LOG2E);
         float o = 0.f;
         if (kd_on) o = akd * et - ckd * pv;
         if (ce_on) o += ace * e1 - cce * hot;
         return o;
     };
-    for (int v = tid; v < a.vocab; v += 256) dz[v] = ElemTraits<T>::from_float(grad(ElemTraits<T>::to_float(z[v]), 0.f, 0.f));
+    for (int v = tid; v < a.vocab; v += NT) dz[v] = ElemTraits<T>::from_float(grad(ElemTraits<T>::to_float(z[v]), 0.f, 0.f));
     __syncthreads();                                     // the row's stores are done: its entries and the label are written again
-    for (int j = tid; j <= a.top; j += 256) {
+    for (int j = tid; j <= a.top; j += NT) {
         const int v = s_i[j];
         if (v < 0) continue;
         float pv = 0.f;
@@ -204,12 +212,263 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillArgs a) {
     }
 }
 
+template <typename T, typename TV>
+__global__ __launch_bounds__(256) void distill_any_kernel(DistillArgs a) {
+    const long long r = blockIdx.x;
+    if ((a.flags & SUBREG_DISTILL_SKIP_UNIT) && a.gs[r * a.gs_stride] == 1.f) return;
+    distill_any_row<T, TV, 256>(a, r);
+}
+
+// NT threads per row, NV loads of 16 bytes a thread in registers.  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
+// labels).  The first wave does the teacher's side while the others' loads are in flight.
+template <typename T, typename TV, int NT, int NV, int SQ>
+__global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
+    using V = RowVec<T>;
+    constexpr int N = V::N, EPL = SUBREG_TOP_MAX / 64;              // entries a lane
+    __shared__ float red[16], red1[16];
+    __shared__ float s_p[SUBREG_TOP_MAX + 1];
+    __shared__ int s_i[SUBREG_TOP_MAX + 1];          // vocabulary entry, -1: none; the label is entry `top`
+    __shared__ float s_cnt[2];
+    const long long r = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float g = a.gs ? a.gs[r * a.gs_stride] : 1.f;
+    if ((a.flags & SUBREG_DISTILL_SKIP_UNIT) && g == 1.f) return;
+    const T* z = (const T*)a.z + r * a.z_stride;
+    T* dz = a.dz ? (T*)a.dz + r * a.vocab : nullptr;
+    const int vocab = a.vocab, top = a.top;
+
+    // which terms the row has (every wave for itself)
+    float tv[EPL];
+    int ti[EPL];
+    bool kept = false, bad = false;
+#pragma unroll
+    for (int q = 0; q < EPL; ++q) {
+        const int j = q * 64 + lane;
+        ti[q] = -1;
+        tv[q] = -INFINITY;
+        if (q * 64 < top) {
+            float v;
+            long long idx;
+            const bool k = entry_kept<TV>(a, r, min(j, top - 1), v, idx) && j < top;
+            kept |= k;
+            bad |= k && idx >= vocab;
+            if (k) { tv[q] = v; ti[q] = idx < vocab ? (int)idx : -1; }
+        }
+    }
+    const bool kd_on = __any(kept);
+    bad = __any(bad);
+    long long y = -1;
+    bool ce_on = false, bad_y = false;
+    if (a.target) {
+        y = a.target[r];
+        ce_on = y != a.ignore;
+        bad_y = ce_on && (y < 0 || y >= vocab);
+        if (!ce_on || bad_y) y = -1;
+    }
+    float* out = a.reduction == SUBREG_NONE ? a.loss : nullptr;
+    if (!kd_on && !ce_on) {
+        if (dz) {
+            V zero;
+            zero.raw = typename V::U{0, 0, 0, 0};
+            for (int c = tid; c * N < vocab; c += NT) zero.store(dz, V::at(c, vocab));
+        }
+        if (tid == 0 && a.loss) {
+            if (out) out[r] = 0.f;
+            else { a.row_kd[r] = 0.f; a.row_ce[r] = 0.f; }
+        }
+        return;
+    }
+    V x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i].load(z, V::at(i * NT + tid, vocab));
+
+    // the teacher's shares (first wave) and the counts (last wave)
+    float p[EPL], tm = -INFINITY, ps = 0.f, z_at[EPL], z_y = 0.f;
+    if (wid == 0) {
+#pragma unroll
+        for (int q = 0; q < EPL; ++q) tm = fmaxf(tm, tv[q]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o));
+#pragma unroll
+        for (int q = 0; q < EPL; ++q) {
+            p[q] = tv[q] == -INFINITY ? 0.f : expf((tv[q] - tm) * a.inv_t);
+            ps += p[q];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) ps += __shfl_xor(ps, o);
+#pragma unroll
+        for (int q = 0; q < EPL; ++q) {
+            const int j = q * 64 + lane;
+            p[q] = kd_on ? p[q] / ps : 0.f;
+            z_at[q] = 0.f;
+            if (j < top) {
+                s_p[j] = p[q];
+                s_i[j] = ti[q];
+                if (ti[q] >= 0) z_at[q] = ElemTraits<T>::to_float(z[ti[q]]);
+            }
+        }
+        if (y >= 0) z_y = ElemTraits<T>::to_float(z[y]);
+        if (lane == 0) {
+            s_p[top] = 0.f;
+            s_i[top] = (int)y;
+        }
+    }
+    if (wid == NT / 64 - 1 && dz) {
+        int n_kd = 0, n_ce = 0;
+        if (a.reduction == SUBREG_MEAN) {
+            for (int b = lane; b < a.count_blocks; b += 64) {
+                n_kd += a.counts[2 * b];
+                n_ce += a.counts[2 * b + 1];
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                n_kd += __shfl_xor(n_kd, o);
+                n_ce += __shfl_xor(n_ce, o);
+            }
+        }
+        if (lane == 0) {
+            s_cnt[0] = (float)max(n_kd, 1);
+            s_cnt[1] = (float)max(n_ce, 1);
+        }
+    }
+
+    // the student's softmax
+    auto add = [](float p, float q) { return p + q; };
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, x[i].get(e));
+    m = block_reduce(m, red, -INFINITY, [](float p, float q) { return fmaxf(p, q); });
+    const float mc = m * a.c_t, mc1 = m * LOG2E;
+    if (!(fabsf(mc) <= 1e30f && fabsf(mc1) <= 1e30f)) {
+        if constexpr (NT >= SUBREG_TOP_MAX) {
+            distill_any_row<T, TV, NT>(a, r);
+            return;
+        }
+    }
+    auto exps = [&](float v, float& et, float& e1) {                // e1 only where a label asks for it
+        et = exp2_fast(fmaf(v, a.c_t, -mc));
+        if constexpr (SQ < 0) {
+            e1 = exp2_fast(fmaf(v, LOG2E, -mc1));
+        } else {
+            e1 = et;
+#pragma unroll
+            for (int k = 0; k < SQ; ++k) e1 *= e1;
+        }
+    };
+    float se = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        x[i].forget();
+        if ((i + 1) * NT * N <= vocab) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float et, e1;
+                exps(x[i].get(e), et, e1);
+                se += et;
+                if constexpr (SQ != 0) s1 += e1;
+            }
+        } else {
+            const int skip = V::skip(i * NT + tid, vocab);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                float et, e1;
+                exps(x[i].get(e), et, e1);
+                se += e >= skip ? et : 0.f;
+                if constexpr (SQ != 0) s1 += e >= skip ? e1 : 0.f;
+            }
+        }
+    }
+    se = block_reduce(se, red, 0.f, add);
+    s1 = SQ == 0 ? se : block_reduce(s1, red1, 0.f, add);
+
+    constexpr float LN2 = 0.69314718055994530942f;
+    if (a.loss && wid == 0) {
+        const float ls = log2f(se), lp = log2f(ps);
+        float term = 0.f;
+#pragma unroll
+        for (int q = 0; q < EPL; ++q)
+            if (p[q] > 0.f || p[q] != p[q])
+                term += p[q] * (((tv[q] - tm) * a.c_t - lp) - (fmaf(z_at[q], a.c_t, -mc) - ls)) * LN2;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) term += __shfl_xor(term, o);
+        if (lane == 0) {
+            if (bad) term = NAN;
+            float ce = 0.f;
+            if (ce_on) {
+                const float xy = SQ < 0 ? fmaf(z_y, LOG2E, -mc1) : fmaf(z_y, a.c_t, -mc) * (float)(1 << (SQ < 0 ? 0 : SQ));
+                ce = bad_y ? NAN : (log2f(s1) - xy) * LN2;
+            }
+            if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
+            else { a.row_kd[r] = term; a.row_ce[r] = ce; }
+        }
+    }
+    if (!dz) return;
+    const float ckd = bad ? NAN : kd_on ? g * a.kd * a.temp / s_cnt[0] : 0.f;
+    const float cce = bad_y ? NAN : ce_on ? g * a.ce / s_cnt[1] : 0.f;
+    const float akd = ckd / se, ace = cce / s1;          // (a term that the row does not have: 0)
+    int tid_again = tid;
+    asm volatile("" : "+v"(tid_again));                  // (the stores' offsets are made where they are used)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = i * NT + tid_again;
+        x[i].forget();
+        typename V::V o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float et, e1;
+            exps(x[i].get(e), et, e1);
+            o[e] = ElemTraits<T>::from_float(SQ == 0 ? (akd + ace) * et : fmaf(ace, e1, akd * et));
+        }
+        V w;
+        w.raw = __builtin_bit_cast(typename V::U, o);
+        if (c * N < vocab) w.store(dz, V::at(c, vocab));             // (where loads overlap, the same values twice)
+    }
+    __syncthreads();                                     // the row's stores are done: its entries and the label are written again
+    for (int j = tid; j <= top; j += NT) {
+        const int v = s_i[j];
+        if (v < 0) continue;
+        float pv = 0.f;
+        bool first = true;
+        for (int i = 0; i <= top; ++i)
+            if (s_i[i] == v) {
+                if (i < j) first = false;
+                pv += s_p[i];
+            }
+        if (!first) continue;
+        float et, e1, o = 0.f;
+        exps(ElemTraits<T>::to_float(z[v]), et, e1);
+        o = akd * et - ckd * pv;
+        o += ace * e1 - (v == (int)y ? cce : 0.f);
+        dz[v] = ElemTraits<T>::from_float(o);
+    }
+}
+
+template <typename T, typename TV, int SQ>
+static void launch_rows(const DistillArgs& a, hipStream_t s) {
+    const long long loads = ((long long)a.vocab + RowVec<T>::N - 1) / RowVec<T>::N;
+#define SUBREG_ROWS(NT, NV) hipLaunchKernelGGL((distill_row_kernel<T, TV, NT, NV, SQ>), a.rows, NT, 0, s, a)
+    if (a.vocab < RowVec<T>::N || loads > 1024 * 16 || loads <= 64) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
+    else if (loads <= 256 * 4) SUBREG_ROWS(256, 4);
+    else if (loads <= 256 * 8) SUBREG_ROWS(256, 8);
+    else if (loads <= 256 * 16) SUBREG_ROWS(256, 16);
+    else if (loads <= 512 * 16) SUBREG_ROWS(512, 16);
+    else SUBREG_ROWS(1024, 16);
+#undef SUBREG_ROWS
+}
+
 template <typename TZ>
 static int distill_launch(const DistillArgs& a, int values_dtype, hipStream_t s) {
     const bool count = a.reduction == SUBREG_MEAN && !(a.flags & SUBREG_DISTILL_COUNTED);
     SUBREG_FOR_FLOAT(values_dtype, {
         if (count) hipLaunchKernelGGL(distill_count_kernel<T>, a.count_blocks, 256, 0, s, a);
-        hipLaunchKernelGGL((distill_row_kernel<TZ, T>), a.rows, 256, 0, s, a);
+        switch (a.target ? a.squarings : 0) {
+            case 0: launch_rows<TZ, T, 0>(a, s); break;
+            case 1: launch_rows<TZ, T, 1>(a, s); break;
+            case 2: launch_rows<TZ, T, 2>(a, s); break;
+            default: launch_rows<TZ, T, -1>(a, s); break;
+        }
     })
     if (a.loss && a.reduction != SUBREG_NONE) hipLaunchKernelGGL(distill_finish_kernel, 1, 1024, 0, s, a);
     return launch_status();
@@ -223,8 +482,7 @@ static inline long long distill_align(long long b) { return (b + 255) / 256 * 25
 
 extern "C" long long subreg_distill_ws_bytes(int rows) {
     if (rows <= 0) return SUBREG_EINVAL;
-    const long long blocks = ((long long)rows + COUNT_ROWS - 1) / COUNT_ROWS;
-    return 2 * distill_align(4ll * rows) + distill_align(8 * blocks);
+    return 2 * distill_align(4ll * rows) + distill_align(8 * COUNT_BLOCKS);
 }
 
 extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
@@ -239,8 +497,9 @@ extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     a.z = d->logits; a.tv = d->top_values; a.ti = d->top_indices; a.target = d->target;
     a.z_stride = d->logits_stride; a.tv_stride = d->values_stride; a.ti_stride = d->indices_stride; a.ignore = d->ignore_index;
     a.rows = d->rows; a.vocab = d->vocab; a.top = d->top; a.reduction = d->reduction; a.flags = d->flags;
-    a.same_t = d->temperature == 1.f;
-    a.count_blocks = (int)(((long long)d->rows + COUNT_ROWS - 1) / COUNT_ROWS);
+    a.squarings = d->temperature == 1.f ? 0 : d->temperature == 2.f ? 1 : d->temperature == 4.f ? 2 : -1;
+    a.count_rows = (int)((((long long)d->rows + COUNT_BLOCKS - 1) / COUNT_BLOCKS + 3) / 4 * 4);
+    a.count_blocks = (int)(((long long)d->rows + a.count_rows - 1) / a.count_rows);
     a.temp = d->temperature; a.inv_t = 1.f / d->temperature; a.c_t = (float)(1.4426950408889634 / (double)d->temperature);
     a.kd = d->kd_weight; a.ce = d->ce_weight;
     a.gs = d->grad_scale; a.gs_stride = d->grad_scale_stride; a.loss = d->loss; a.dz = d->dlogits;

@@ -51,8 +51,10 @@ template <typename T> struct RowVec {
     U raw;
     static __device__ __forceinline__ int at(int c, int n) { return min(c * N, n - N); }
     static __device__ __forceinline__ int skip(int c, int n) { return max(c * N - (n - N), 0); }
-    __device__ __forceinline__ void load(const T* row, int at) { __builtin_memcpy(&raw, row + at, 16); }
-    __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy(row + at, &raw, 16); }
+    // (a 32-bit byte offset from the row's address, which all lanes share: one register a load in flight, not two)
+    static __device__ __forceinline__ unsigned bytes(int at) { return (unsigned)at * (unsigned)sizeof(T); }
+    __device__ __forceinline__ void load(const T* row, int at) { __builtin_memcpy(&raw, (const char*)row + bytes(at), 16); }
+    __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy((char*)row + bytes(at), &raw, 16); }
     __device__ __forceinline__ T elem(int e) const { return __builtin_bit_cast(V, raw)[e]; }
     __device__ __forceinline__ float get(int e) const { return ElemTraits<T>::to_float(elem(e)); }
     // between two uses of a held row: what the first use unpacked is unpacked again (kept, it would take twice the registers)

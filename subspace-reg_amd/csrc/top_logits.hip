@@ -31,7 +31,7 @@ template <typename T, unsigned INF> struct TopKey16 {
 template <> struct TopKey<__bf16> : TopKey16<__bf16, 0x7f80u> {};
 template <> struct TopKey<_Float16> : TopKey16<_Float16, 0x7c00u> {};
 
-// One block per row (or part of one), the row read once:
+// One block per row, the row read once:
 //   1. every thread keeps the largest logit of what it read;
 //   2. a wave finds a key t that at least `top` threads' maxima reach, so at least `top` logits do (bit by bit over the NT maxima; stops
 //      as soon as between top and 2 top of them reach it);
@@ -54,20 +54,13 @@ __device__ __forceinline__ int lds_add(int* p, int n) {
     return old;
 }
 
-// Where a block's selection goes: the row's answer, or (PART: the block had a part of a long row) pairs for join_kernel
-template <typename T, bool PART> struct TopOut {
+// the row's answer
+template <typename T> struct TopOut {
     T* values;
     long long* indices;
-    u64* pairs;
-    int base;                                         // index of row[0] in the whole row
     __device__ __forceinline__ void put(int place, u64 me) const {
-        const unsigned v = 0xffffffffu - (unsigned)me;
-        if constexpr (PART) {
-            pairs[place] = (me & 0xffffffff00000000ull) | (0xffffffffu - (v + (unsigned)base));
-        } else {
-            values[place] = TopKey<T>::value((unsigned)(me >> 32));
-            indices[place] = v;
-        }
+        values[place] = TopKey<T>::value((unsigned)(me >> 32));
+        indices[place] = 0xffffffffu - (unsigned)me;
     }
 };
 
@@ -171,11 +164,10 @@ template <typename T> struct TopSeen {
     __device__ __forceinline__ bool others_reach(unsigned t) const { return nan() || TopKey<T>::of(ElemTraits<T>::from_float(second)) >= t; }
 };
 
-template <typename T, int NT, bool PART>
-__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_logits_kernel(const T* __restrict__ z, long long stride, int vocab_all,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_logits_kernel(const T* __restrict__ z, long long stride, int vocab,
                                                                             int top, T* __restrict__ values,
-                                                                            long long* __restrict__ indices, u64* __restrict__ pairs,
-                                                                            int part_len) {
+                                                                            long long* __restrict__ indices) {
     using V = RowVec<T>;
     constexpr int N = V::N, DEEP = 8;                 // loads a thread has in flight
     __shared__ int red[16];
@@ -187,9 +179,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_logits_kernel(cons
     __shared__ unsigned border;
     const long long r = blockIdx.x;
     const int tid = threadIdx.x;
-    const int v0 = PART ? (int)blockIdx.y * part_len : 0, vocab = PART ? min(part_len, vocab_all - v0) : vocab_all;
-    const T* row = z + r * stride + v0;
-    const TopOut<T, PART> out{values + r * top, indices + r * top, pairs + (r * gridDim.y + blockIdx.y) * top, v0};
+    const T* row = z + r * stride;
+    const TopOut<T> out{values + r * top, indices + r * top};
     const int loads = (vocab + N - 1) / N;
 
     TopSeen<T> seen;
@@ -295,33 +286,6 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_logits_kernel(cons
     else write_places<NT>(list, n, top, out);
 }
 
-// The `top` best of a row from the sorted pairs of its `parts` parts.  The part that holds least decides a border: with q =
-// ceil(top / parts), at least parts q >= top pairs are as large as the smallest of the parts' q-th.
-template <typename T>
-__global__ __launch_bounds__(512) void top_join_kernel(const u64* __restrict__ pairs, int parts, int top, T* __restrict__ values,
-                                                       long long* __restrict__ indices) {
-    extern __shared__ __attribute__((aligned(16))) u64 list_join[];
-    __shared__ int filled;
-    const long long r = blockIdx.x;
-    const u64* p = pairs + r * parts * top;
-    const TopOut<T, false> out{values + r * top, indices + r * top, nullptr, 0};
-    if (threadIdx.x == 0) filled = 0;
-    const int lane = threadIdx.x & 63;                // every wave finds the border for itself (parts <= 32)
-    u64 t = p[(long long)min(lane, parts - 1) * top + (top + parts - 1) / parts - 1];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 v = __shfl_xor(t, o);
-        t = v < t ? v : t;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < parts * top; i += 512) {
-        const u64 v = p[i];
-        if (v >= t) list_join[atomicAdd(&filled, 1)] = v;
-    }
-    __syncthreads();
-    write_places<512>(list_join, filled, top, out);
-}
-
 // short rows: one wave per row, its keys in registers
 template <typename T>
 __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ z, long long stride, int rows, int vocab, int top,
@@ -350,7 +314,7 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ z,
         }
     }
     t = max(t, 1u);
-    const TopOut<T, false> out{values + r * top, indices + r * top, nullptr, 0};
+    const TopOut<T> out{values + r * top, indices + r * top};
     u64* list = lists[w];
     int n = 0;
 #pragma unroll
@@ -369,36 +333,22 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ z,
     }
 }
 
-// Parts of a row: few long rows leave most of the chip idle, so each is cut for up to 32 blocks and joined by a second launch.
-// (A join holds parts x top pairs in LDS: at most 4096.)
-static int top_parts(int rows, int vocab, int top) {
-    long long p = vocab / 4096;
-    const long long most[3] = {256 / (long long)rows, 32, 4096 / top};
-    for (long long m : most) p = p < m ? p : m;
-    return p < 4 ? 1 : (int)p;
-}
-
 template <typename T>
-static int launch_top(const T* z, long long stride, int rows, int vocab, int top, T* values, long long* indices, u64* ws, hipStream_t s) {
-    const int parts = top_parts(rows, vocab, top);
-    const int len = parts == 1 ? vocab : ((vocab + parts - 1) / parts + 7) / 8 * 8;
-    const long long loads = ((long long)len + RowVec<T>::N - 1) / RowVec<T>::N;
-#define SUBREG_TOP(NT, PART) \
-    hipLaunchKernelGGL((top_logits_kernel<T, NT, PART>), dim3(rows, parts), NT, 0, s, z, stride, vocab, top, values, indices, ws, len)
-    // threads: twice `top` at least (their maxima are what the border is found among), and at most 32 loads each
-    const int nt = loads > 512 * 32 ? 1024 : loads > 256 * 32 || top > 128 ? 512 : 256;
-    if (parts > 1) {
-        if (nt == 256) SUBREG_TOP(256, true);
-        else if (nt == 512) SUBREG_TOP(512, true);
-        else SUBREG_TOP(1024, true);
-        hipLaunchKernelGGL(top_join_kernel<T>, rows, 512, sizeof(u64) * (parts * top + 8), s, ws, parts, top, values, indices);
-    } else if (vocab <= TOP_SHORT) {
+static int launch_top(const T* z, long long stride, int rows, int vocab, int top, T* values, long long* indices, hipStream_t s) {
+    const long long loads = ((long long)vocab + RowVec<T>::N - 1) / RowVec<T>::N;
+    if (vocab <= TOP_SHORT) {
         hipLaunchKernelGGL(top_short_kernel<T>, (int)(((long long)rows + 3) / 4), 256, 0, s, z, stride, rows, vocab, top, values, indices);
-    } else {
-        if (nt == 256) SUBREG_TOP(256, false);
-        else if (nt == 512) SUBREG_TOP(512, false);
-        else SUBREG_TOP(1024, false);
+        return launch_status();
     }
+#define SUBREG_TOP(NT) hipLaunchKernelGGL((top_logits_kernel<T, NT>), rows, NT, 0, s, z, stride, vocab, top, values, indices)
+    // Threads: twice `top` at least (the border is found among their maxima), at most 32 loads each, and 16 where there is a block per
+    // CU at most, so that a row's latency counts: 1 row of 50000 bf16 takes 11.0 | 8.8 | 9.8 us on 256 | 512 | 1024 threads, of 32000
+    // 7.6 | 7.5 | 10.3, of 128000 15.8 | 10.8 | 11.2.  (A row cut into 16 parts for as many blocks and joined by a second launch: 11.2 -
+    // 12.5 us for all of these.)
+    const bool few = rows <= 256;
+    if (loads > 512 * 32) SUBREG_TOP(1024);
+    else if (loads > 256 * (few ? 16 : 32) || top > 128) SUBREG_TOP(512);
+    else SUBREG_TOP(256);
 #undef SUBREG_TOP
     return launch_status();
 }
@@ -407,19 +357,10 @@ static int launch_top(const T* z, long long stride, int rows, int vocab, int top
 
 using namespace subreg;
 
-extern "C" long long subreg_top_logits_ws_bytes(int rows, int vocab, int top) {
-    if (rows <= 0 || vocab <= 0 || vocab > MAX_COLUMNS || top < 1 || top > vocab || top > SUBREG_TOP_MAX) return SUBREG_EINVAL;
-    const long long parts = top_parts(rows, vocab, top);
-    return parts == 1 ? 0 : (long long)sizeof(u64) * rows * parts * top;
-}
-
 extern "C" int subreg_top_logits(const void* logits, long long stride, int dtype, int rows, int vocab, int top, void* values,
-                                 long long* indices, void* ws, long long ws_bytes, void* stream) {
+                                 long long* indices, void* stream) {
     SUBREG_CHECK_ARG(logits && values && indices && rows > 0 && vocab > 0 && vocab <= MAX_COLUMNS && stride >= 0);
     SUBREG_CHECK_ARG(top >= 1 && top <= vocab && top <= SUBREG_TOP_MAX);
-    const long long need = subreg_top_logits_ws_bytes(rows, vocab, top);
-    SUBREG_CHECK_ARG(need == 0 || (ws && ((size_t)ws & 255) == 0 && ws_bytes >= need));
-    SUBREG_FOR_FLOAT(dtype, return launch_top<T>((const T*)logits, stride, rows, vocab, top, (T*)values, indices, (u64*)ws,
-                                                 (hipStream_t)stream))
+    SUBREG_FOR_FLOAT(dtype, return launch_top<T>((const T*)logits, stride, rows, vocab, top, (T*)values, indices, (hipStream_t)stream))
     return SUBREG_EINVAL;
 }

@@ -172,8 +172,7 @@ SIGNATURES = {
     "subreg_quantize_rows": (_I, [_P, _L, _I, _I, _I, _P, _L, _P, _P]),
     "subreg_linear_int8_ws_bytes": (_L, [_I, _I, _I, _I, _P, _L]),
     "subreg_linear_int8": (_I, [_P, _L, _I, _P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P]),
-    "subreg_top_logits_ws_bytes": (_L, [_I, _I, _I]),
-    "subreg_top_logits": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P, _L, _P]),
+    "subreg_top_logits": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P]),
     "subreg_distill_ws_bytes": (_L, [_I]),
     "subreg_distill_loss": (_I, [C.POINTER(DistillDesc), _P]),
 }

@@ -342,11 +342,8 @@ def top_logits(logits, k):
     values = torch.empty(shape, dtype=logits.dtype, device=dev)
     indices = torch.empty(shape, dtype=torch.int64, device=dev)
     if n:
-        lib = _lib.load()
-        nbytes = lib.subreg_top_logits_ws_bytes(n, vocab, k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _launch(dev, lib.subreg_top_logits, "top_logits", rows.data_ptr(), rows.stride(0), code, n, vocab, k, values.data_ptr(),
-                indices.data_ptr(), _ptr(ws), nbytes)
+        _launch(dev, _lib.load().subreg_top_logits, "top_logits", rows.data_ptr(), rows.stride(0), code, n, vocab, k, values.data_ptr(),
+                indices.data_ptr())
     return values, indices
 
 

@@ -189,12 +189,9 @@ def test_c_entries_refuse_on_cpu():
         bad = list(args)
         bad[at] = value
         assert lib.subreg_linear_int8(*bad) == -1, at
-    assert lib.subreg_top_logits_ws_bytes(64, 1000, 5) == 0 and lib.subreg_top_logits_ws_bytes(1, 8, 9) == -1
-    n = lib.subreg_top_logits_ws_bytes(1, 100000, 5)
-    for bad in ((None, 8, 0, 1, 8, 1, p, p, None, 0, None), (p, 8, 0, 1, 8, 9, p, p, None, 0, None), (p, 300, 0, 1, 300, 257, p, p, None, 0, None),
-                (p, 8, 3, 1, 8, 1, p, p, None, 0, None), (p, -1, 0, 1, 8, 1, p, p, None, 0, None), (p, 8, 0, 0, 8, 1, p, p, None, 0, None),
-                (p, 8, 0, 1, 100000, 5, p, p, None, n, None), (p, 8, 0, 1, 100000, 5, p, p, p + 8, n, None),
-                (p, 8, 0, 1, 100000, 5, p, p, p, n - 1, None)):
+    for bad in ((None, 8, 0, 1, 8, 1, p, p, None), (p, 8, 0, 1, 8, 9, p, p, None), (p, 300, 0, 1, 300, 257, p, p, None),
+                (p, 8, 3, 1, 8, 1, p, p, None), (p, -1, 0, 1, 8, 1, p, p, None), (p, 8, 0, 0, 8, 1, p, p, None),
+                (p, 8, 0, 1, (1 << 30) + 1, 1, p, p, None)):
         assert lib.subreg_top_logits(*bad) == -1
     assert lib.subreg_distill_ws_bytes(0) == -1
 
