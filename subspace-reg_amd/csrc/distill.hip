@@ -35,6 +35,13 @@ struct DistillArgs {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// a product that is rounded: the difference of two such is 0 where they are equal (fused with the subtraction it would be the rounding
+// error of one of them, which for masked rows' maxima is large)
+__device__ __forceinline__ float rounded_product(float x, float y) {
+#pragma clang fp contract(off)
+    return x * y;
+}
+
 template <typename TV>
 __device__ __forceinline__ bool entry_kept(const DistillArgs& a, long long r, int j, float& v, long long& idx) {
     idx = a.ti[r * a.ti_stride + j];
@@ -219,7 +226,8 @@ __global__ __launch_bounds__(256) void distill_any_kernel(DistillArgs a) {
     distill_any_row<T, TV, 256>(a, r);
 }
 
-// NT threads per row, NV loads of 16 bytes a thread in registers.  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
+// NT threads per row, NV loads of 16 bytes a thread in registers; NV = 0: the loss alone, the row streamed with a running maximum and sum
+// a thread (few registers: eight blocks a CU, any length).  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
 // labels).  The first wave does the teacher's side while the others' loads are in flight.
 template <typename T, typename TV, int NT, int NV, int SQ>
 __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
         }
         return;
     }
-    V x[NV];
+    V x[NV ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i].load(z, V::at(i * NT + tid, vocab));
 
@@ -334,20 +342,8 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
 
     // the student's softmax
     auto add = [](float p, float q) { return p + q; };
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) m = fmaxf(m, x[i].get(e));
-    m = block_reduce(m, red, -INFINITY, [](float p, float q) { return fmaxf(p, q); });
-    const float mc = m * a.c_t, mc1 = m * LOG2E;
-    if (!(fabsf(mc) <= 1e30f && fabsf(mc1) <= 1e30f)) {
-        if constexpr (NT >= SUBREG_TOP_MAX) {
-            distill_any_row<T, TV, NT>(a, r);
-            return;
-        }
-    }
-    auto exps = [&](float v, float& et, float& e1) {                // e1 only where a label asks for it
+    auto larger = [](float p, float q) { return fmaxf(p, q); };
+    auto exps = [&](float v, float mc, float mc1, float& et, float& e1) {
         et = exp2_fast(fmaf(v, a.c_t, -mc));
         if constexpr (SQ < 0) {
             e1 = exp2_fast(fmaf(v, LOG2E, -mc1));
@@ -358,27 +354,69 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
         }
     };
     float se = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        x[i].forget();
-        if ((i + 1) * NT * N <= vocab) {
+    // load c (of thread 0: first) into the sums; elements that another load covers count 0
+    auto sum = [&](V& l, int first, int c, float mc, float mc1) {
+        l.forget();
+        if ((first + NT) * N <= vocab) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 float et, e1;
-                exps(x[i].get(e), et, e1);
+                exps(l.get(e), mc, mc1, et, e1);
                 se += et;
                 if constexpr (SQ != 0) s1 += e1;
             }
         } else {
-            const int skip = V::skip(i * NT + tid, vocab);
+            const int skip = V::skip(c, vocab);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 float et, e1;
-                exps(x[i].get(e), et, e1);
+                exps(l.get(e), mc, mc1, et, e1);
                 se += e >= skip ? et : 0.f;
                 if constexpr (SQ != 0) s1 += e >= skip ? e1 : 0.f;
             }
         }
+    };
+    // (a running maximum starts at a floor whose product with c is a number, so that masked logits of -infinity add 0)
+    const float floor_m = -1e30f / fmaxf(a.c_t, 1.f);
+    float m = NV ? -INFINITY : floor_m;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) m = fmaxf(m, x[i].get(e));
+    } else {
+        constexpr int DEEP = 4;
+        const int loads = (vocab + N - 1) / N;
+        for (int c0 = 0; c0 < loads; c0 += DEEP * NT) {
+            V l[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) l[i].load(z, V::at(c0 + i * NT + tid, vocab));
+            const float mc_was = rounded_product(m, a.c_t), mc1_was = rounded_product(m, LOG2E);
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) m = fmaxf(m, l[i].get(e));
+            const float mc = rounded_product(m, a.c_t), mc1 = rounded_product(m, LOG2E);
+            se *= exp2_fast(mc_was - mc);
+            if constexpr (SQ != 0) s1 *= exp2_fast(SQ < 0 ? mc1_was - mc1 : (mc_was - mc) * (float)(1 << max(SQ, 0)));
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if ((c0 + i * NT) < loads) sum(l[i], c0 + i * NT, c0 + i * NT + tid, mc, mc1);
+        }
+    }
+    const float mc_own = rounded_product(m, a.c_t), mc1_own = rounded_product(m, LOG2E);
+    m = block_reduce(m, red, -INFINITY, larger);
+    const float mc = rounded_product(m, a.c_t), mc1 = rounded_product(m, LOG2E);
+    if (!(m > floor_m && fabsf(mc) <= 1e30f && fabsf(mc1) <= 1e30f)) {
+        distill_any_row<T, TV, NT>(a, r);
+        return;
+    }
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sum(x[i], i * NT, i * NT + tid, mc, mc1);
+    } else {
+        se *= exp2_fast(mc_own - mc);
+        if constexpr (SQ != 0) s1 *= exp2_fast(SQ < 0 ? mc1_own - mc1 : (mc_own - mc) * (float)(1 << max(SQ, 0)));
     }
     se = block_reduce(se, red, 0.f, add);
     s1 = SQ == 0 ? se : block_reduce(s1, red1, 0.f, add);
@@ -397,51 +435,52 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
             if (bad) term = NAN;
             float ce = 0.f;
             if (ce_on) {
-                const float xy = SQ < 0 ? fmaf(z_y, LOG2E, -mc1) : fmaf(z_y, a.c_t, -mc) * (float)(1 << (SQ < 0 ? 0 : SQ));
+                const float xy = SQ < 0 ? fmaf(z_y, LOG2E, -mc1) : fmaf(z_y, a.c_t, -mc) * (float)(1 << max(SQ, 0));
                 ce = bad_y ? NAN : (log2f(s1) - xy) * LN2;
             }
             if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
             else { a.row_kd[r] = term; a.row_ce[r] = ce; }
         }
     }
-    if (!dz) return;
-    const float ckd = bad ? NAN : kd_on ? g * a.kd * a.temp / s_cnt[0] : 0.f;
-    const float cce = bad_y ? NAN : ce_on ? g * a.ce / s_cnt[1] : 0.f;
-    const float akd = ckd / se, ace = cce / s1;          // (a term that the row does not have: 0)
-    int tid_again = tid;
-    asm volatile("" : "+v"(tid_again));                  // (the stores' offsets are made where they are used)
+    if constexpr (NV > 0) {
+        const float ckd = bad ? NAN : kd_on ? g * a.kd * a.temp / s_cnt[0] : 0.f;
+        const float cce = bad_y ? NAN : ce_on ? g * a.ce / s_cnt[1] : 0.f;
+        const float akd = ckd / se, ace = cce / s1;          // (a term that the row does not have: 0)
+        int tid_again = tid;
+        asm volatile("" : "+v"(tid_again));                  // (the stores' offsets are made where they are used)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = i * NT + tid_again;
-        x[i].forget();
-        typename V::V o;
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * NT + tid_again;
+            x[i].forget();
+            typename V::V o;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            float et, e1;
-            exps(x[i].get(e), et, e1);
-            o[e] = ElemTraits<T>::from_float(SQ == 0 ? (akd + ace) * et : fmaf(ace, e1, akd * et));
-        }
-        V w;
-        w.raw = __builtin_bit_cast(typename V::U, o);
-        if (c * N < vocab) w.store(dz, V::at(c, vocab));             // (where loads overlap, the same values twice)
-    }
-    __syncthreads();                                     // the row's stores are done: its entries and the label are written again
-    for (int j = tid; j <= top; j += NT) {
-        const int v = s_i[j];
-        if (v < 0) continue;
-        float pv = 0.f;
-        bool first = true;
-        for (int i = 0; i <= top; ++i)
-            if (s_i[i] == v) {
-                if (i < j) first = false;
-                pv += s_p[i];
+            for (int e = 0; e < N; ++e) {
+                float et, e1;
+                exps(x[i].get(e), mc, mc1, et, e1);
+                o[e] = ElemTraits<T>::from_float(SQ == 0 ? (akd + ace) * et : fmaf(ace, e1, akd * et));
             }
-        if (!first) continue;
-        float et, e1, o = 0.f;
-        exps(ElemTraits<T>::to_float(z[v]), et, e1);
-        o = akd * et - ckd * pv;
-        o += ace * e1 - (v == (int)y ? cce : 0.f);
-        dz[v] = ElemTraits<T>::from_float(o);
+            V w;
+            w.raw = __builtin_bit_cast(typename V::U, o);
+            if (c * N < vocab) w.store(dz, V::at(c, vocab));             // (where loads overlap, the same values twice)
+        }
+        __syncthreads();                                     // the row's stores are done: its entries and the label are written again
+        for (int j = tid; j <= top; j += NT) {
+            const int v = s_i[j];
+            if (v < 0) continue;
+            float pv = 0.f;
+            bool first = true;
+            for (int i = 0; i <= top; ++i)
+                if (s_i[i] == v) {
+                    if (i < j) first = false;
+                    pv += s_p[i];
+                }
+            if (!first) continue;
+            float et, e1, o = 0.f;
+            exps(ElemTraits<T>::to_float(z[v]), mc, mc1, et, e1);
+            o = akd * et - ckd * pv;
+            o += ace * e1 - (v == (int)y ? cce : 0.f);
+            dz[v] = ElemTraits<T>::from_float(o);
+        }
     }
 }
 
@@ -449,7 +488,8 @@ template <typename T, typename TV, int SQ>
 static void launch_rows(const DistillArgs& a, hipStream_t s) {
     const long long loads = ((long long)a.vocab + RowVec<T>::N - 1) / RowVec<T>::N;
 #define SUBREG_ROWS(NT, NV) hipLaunchKernelGGL((distill_row_kernel<T, TV, NT, NV, SQ>), a.rows, NT, 0, s, a)
-    if (a.vocab < RowVec<T>::N || loads > 1024 * 16 || loads <= 64) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
+    if (a.vocab < RowVec<T>::N || loads <= 64 || (a.dz && loads > 1024 * 16)) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
+    else if (!a.dz) SUBREG_ROWS(256, 0);
     else if (loads <= 256 * 4) SUBREG_ROWS(256, 4);
     else if (loads <= 256 * 8) SUBREG_ROWS(256, 8);
     else if (loads <= 256 * 16) SUBREG_ROWS(256, 16);

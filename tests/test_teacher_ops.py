@@ -399,8 +399,9 @@ def check_distill(z, tv, ti, y, temp=1.0, kd=1.0, ce=0.0, reduction="mean", g=No
         elem = elem * float(gg.abs().max())
     assert leaf.grad.dtype == z.dtype and leaf.grad.shape == z.shape
     close(leaf.grad.reshape(-1, z.shape[-1]), grad, elem, z.dtype, "gradient")
-    with torch.no_grad():                                            # the loss alone
-        assert torch.equal(HF.distill_loss(leaf, tv, ti, y, temp, kd, ce, ignore, reduction).nan_to_num(3), loss.detach().nan_to_num(3))
+    with torch.no_grad():                                            # the loss alone: sums in another order, the same bound
+        alone = HF.distill_loss(leaf, tv, ti, y, temp, kd, ce, ignore, reduction)
+    close(alone.reshape(-1), want.reshape(-1), row * (n if reduction == "sum" else 2), note="the loss alone")
     return loss.detach(), leaf.grad
 
 
