@@ -14,6 +14,7 @@
 namespace subreg {
 
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int COUNT_INLINE = 2048;       // up to so many entries every block counts for itself
 constexpr int COUNT_BLOCKS = 256;        // at most, of the counting kernel
 
 struct DistillArgs {
@@ -49,6 +50,30 @@ __device__ __forceinline__ bool entry_kept(const DistillArgs& a, long long r, in
     return idx >= 0 && !(v == -INFINITY);
 }
 
+// a thread's share (thread `tid` of `nt`) of the numbers of rows with entries and with a label: from the counting kernel's sums, or, where
+// the call is so small that every row's entries cost less than another launch, from the entries themselves
+template <typename TV, bool INLINE>
+__device__ __forceinline__ void row_counts(const DistillArgs& a, int tid, int nt, int& n_kd, int& n_ce) {
+    if (!INLINE || a.count_blocks) {
+        for (int b = tid; b < a.count_blocks; b += nt) {
+            n_kd += a.counts[2 * b];
+            n_ce += a.counts[2 * b + 1];
+        }
+        return;
+    }
+    for (int r = tid; r < a.rows; r += nt) {
+        bool any = false;
+#pragma unroll 4
+        for (int j = 0; j < a.top; ++j) {
+            float v;
+            long long idx;
+            any |= entry_kept<TV>(a, r, j, v, idx);
+        }
+        n_kd += any;
+        n_ce += a.target && a.target[r] != a.ignore;
+    }
+}
+
 template <typename TV>
 __global__ __launch_bounds__(256) void distill_count_kernel(DistillArgs a) {
     __shared__ int red[16];
@@ -75,33 +100,44 @@ __global__ __launch_bounds__(256) void distill_count_kernel(DistillArgs a) {
     }
 }
 
-// loss[0] from the rows' terms, in a fixed order
+// loss[0] from the rows' terms, in a fixed order; the rows that have a term are counted by its value (a row without one holds NO_TERM,
+// which no KL and no cross entropy can be)
+constexpr float NO_TERM = -INFINITY;
 __global__ __launch_bounds__(1024) void distill_finish_kernel(DistillArgs a) {
-    __shared__ double red[16];
-    double kd = 0, ce = 0, n_kd = 0, n_ce = 0;
+    __shared__ double red[4][16];
+    double v[4] = {0, 0, 0, 0};
+#pragma unroll 4
     for (int r = threadIdx.x; r < a.rows; r += 1024) {
-        kd += (double)a.row_kd[r];
-        ce += (double)a.row_ce[r];
+        const float kd = a.row_kd[r], ce = a.row_ce[r];
+        if (kd != NO_TERM) { v[0] += (double)kd; v[2] += 1.0; }
+        if (ce != NO_TERM) { v[1] += (double)ce; v[3] += 1.0; }
     }
-    auto add = [](double p, double q) { return p + q; };
-    kd = block_reduce(kd, red, 0.0, add);
-    ce = block_reduce(ce, red, 0.0, add);
-    if (a.reduction == SUBREG_MEAN) {
-        for (int b = threadIdx.x; b < a.count_blocks; b += 1024) {
-            n_kd += a.counts[2 * b];
-            n_ce += a.counts[2 * b + 1];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o);
+        if (lane == 0) red[k][wid] = v[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = red[k][lane & 15];
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o);
         }
-        n_kd = block_reduce(n_kd, red, 0.0, add);
-        n_ce = block_reduce(n_ce, red, 0.0, add);
-        kd /= fmax(n_kd, 1.0);
-        ce /= fmax(n_ce, 1.0);
+        if (lane == 0) {
+            const bool mean = a.reduction == SUBREG_MEAN;
+            const double kd = mean ? v[0] / fmax(v[2], 1.0) : v[0], ce = mean ? v[1] / fmax(v[3], 1.0) : v[1];
+            a.loss[0] = (float)((double)a.kd * a.temp * a.temp * kd + (double)a.ce * ce);
+        }
     }
-    if (threadIdx.x == 0) a.loss[0] = (float)((double)a.kd * a.temp * a.temp * kd + (double)a.ce * ce);
 }
 
 // any row: shorter than a load, longer than the registers hold, or with a maximum so large that m c is not a number to subtract
 // (logits of the type's lowest value, infinities).  NT threads of one row; reads it three times, from the caches after the first.
-template <typename T, typename TV, int NT>
+template <typename T, typename TV, int NT, bool INLINE>
 __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long r) {
     __shared__ float red[16];
     __shared__ int redi[16];
@@ -117,14 +153,17 @@ __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long 
     auto mx = [](float p, float q) { return fmaxf(p, q); };
 
     // the teacher's share
-    float tv = -INFINITY;
-    long long ti = -1;
-    static_assert(NT >= SUBREG_TOP_MAX, "one entry a thread");
-    const bool kept = tid < a.top && entry_kept<TV>(a, r, tid, tv, ti);
-    const bool wild = kept && ti >= a.vocab;
-    const int state = block_reduce((kept ? 1 : 0) + (wild ? 1 << 16 : 0), redi, 0, addi);
-    const bool kd_on = (state & 0xffff) != 0;
-    bool bad = state >> 16 != 0;
+    int state = 0;
+    float tm = -INFINITY;
+    for (int j = tid; j < a.top; j += NT) {
+        float v;
+        long long idx;
+        if (!entry_kept<TV>(a, r, j, v, idx)) continue;
+        state += 1 + (idx >= a.vocab ? 1 << 16 : 0);
+        tm = fmaxf(tm, v);
+    }
+    state = block_reduce(state, redi, 0, addi);
+    const bool kd_on = (state & 0xffff) != 0, bad = state >> 16 != 0;
     long long y = -1;
     bool ce_on = false, bad_y = false;
     if (a.target) {
@@ -136,10 +175,7 @@ __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long 
     float cnt_kd = 1.f, cnt_ce = 1.f;
     if (a.reduction == SUBREG_MEAN && dz) {
         int n_kd = 0, n_ce = 0;
-        for (int b = tid; b < a.count_blocks; b += NT) {
-            n_kd += a.counts[2 * b];
-            n_ce += a.counts[2 * b + 1];
-        }
+        row_counts<TV, INLINE>(a, tid, NT, n_kd, n_ce);
         cnt_kd = (float)max(1, block_reduce(n_kd, redi, 0, addi));
         cnt_ce = (float)max(1, block_reduce(n_ce, redi, 0, addi));
     }
@@ -149,18 +185,22 @@ __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long 
             for (int v = tid; v < a.vocab; v += NT) dz[v] = ElemTraits<T>::from_float(0.f);
         if (tid == 0 && a.loss) {
             if (out) out[r] = 0.f;
-            else { a.row_kd[r] = 0.f; a.row_ce[r] = 0.f; }
+            else { a.row_kd[r] = NO_TERM; a.row_ce[r] = NO_TERM; }
         }
         return;
     }
-    const float tm = block_reduce(kept ? tv : -INFINITY, red, -INFINITY, mx);
-    float p = kept ? expf((tv - tm) * a.inv_t) : 0.f;
-    const float ps = block_reduce(p, red, 0.f, add);
-    p = kd_on ? p / ps : 0.f;
-    if (tid < a.top) {
-        s_p[tid] = p;
-        s_i[tid] = kept && !wild ? (int)ti : -1;
+    tm = block_reduce(tm, red, -INFINITY, mx);
+    float ps = 0.f;
+    for (int j = tid; j < a.top; j += NT) {
+        float v;
+        long long idx;
+        const bool kept = entry_kept<TV>(a, r, j, v, idx);
+        s_p[j] = kept ? expf((v - tm) * a.inv_t) : 0.f;
+        s_i[j] = kept && idx < a.vocab ? (int)idx : -1;
+        ps += s_p[j];
     }
+    ps = block_reduce(ps, red, 0.f, add);
+    for (int j = tid; j < a.top; j += NT) s_p[j] = kd_on ? s_p[j] / ps : 0.f;
     if (tid == 0) {
         s_p[a.top] = 0.f;
         s_i[a.top] = (int)y;
@@ -181,14 +221,18 @@ __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long 
 
     if (a.loss) {
         float term = 0.f;
-        if (kept && !wild && !(p == 0.f))
-            term = p * (((tv - tm) - (ElemTraits<T>::to_float(z[ti]) - m)) * a.inv_t + (logf(se) - logf(ps)));
+        for (int j = tid; j < a.top; j += NT) {
+            const float p = s_p[j];
+            if (s_i[j] < 0 || p == 0.f) continue;
+            const float tv = ElemTraits<TV>::to_float(((const TV*)a.tv)[r * a.tv_stride + j]);
+            term += p * (((tv - tm) - (ElemTraits<T>::to_float(z[s_i[j]]) - m)) * a.inv_t + (logf(se) - logf(ps)));
+        }
         term = block_reduce(term, red, 0.f, add);
         if (tid == 0) {
             if (bad) term = NAN;
             const float ce = !ce_on ? 0.f : bad_y ? NAN : logf(s1) - (ElemTraits<T>::to_float(z[y]) - m);
             if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
-            else { a.row_kd[r] = term; a.row_ce[r] = ce; }
+            else { a.row_kd[r] = kd_on ? term : NO_TERM; a.row_ce[r] = ce_on ? ce : NO_TERM; }
         }
     }
     if (!dz) return;
@@ -223,11 +267,11 @@ template <typename T, typename TV>
 __global__ __launch_bounds__(256) void distill_any_kernel(DistillArgs a) {
     const long long r = blockIdx.x;
     if ((a.flags & SUBREG_DISTILL_SKIP_UNIT) && a.gs[r * a.gs_stride] == 1.f) return;
-    distill_any_row<T, TV, 256>(a, r);
+    distill_any_row<T, TV, 256, true>(a, r);
 }
 
-// NT threads per row, NV loads of 16 bytes a thread in registers; NV = 0: the loss alone, the row streamed with a running maximum and sum
-// a thread (few registers: eight blocks a CU, any length).  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
+// NT threads per row, NV loads of 16 bytes a thread in registers; NV = 0: the row streamed with a running maximum and sum a thread (few
+// registers, any length): the loss alone, and rows that do not fit the registers, which are then read a second time.  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
 // labels).  The first wave does the teacher's side while the others' loads are in flight.
 template <typename T, typename TV, int NT, int NV, int SQ>
 __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
@@ -282,7 +326,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
         }
         if (tid == 0 && a.loss) {
             if (out) out[r] = 0.f;
-            else { a.row_kd[r] = 0.f; a.row_ce[r] = 0.f; }
+            else { a.row_kd[r] = NO_TERM; a.row_ce[r] = NO_TERM; }
         }
         return;
     }
@@ -324,10 +368,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     if (wid == NT / 64 - 1 && dz) {
         int n_kd = 0, n_ce = 0;
         if (a.reduction == SUBREG_MEAN) {
-            for (int b = lane; b < a.count_blocks; b += 64) {
-                n_kd += a.counts[2 * b];
-                n_ce += a.counts[2 * b + 1];
-            }
+            row_counts<TV, NT == 64>(a, lane, 64, n_kd, n_ce);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
                 n_kd += __shfl_xor(n_kd, o);
@@ -408,7 +449,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     m = block_reduce(m, red, -INFINITY, larger);
     const float mc = rounded_product(m, a.c_t), mc1 = rounded_product(m, LOG2E);
     if (!(m > floor_m && fabsf(mc) <= 1e30f && fabsf(mc1) <= 1e30f)) {
-        distill_any_row<T, TV, NT>(a, r);
+        distill_any_row<T, TV, NT, NT == 64>(a, r);
         return;
     }
     if constexpr (NV > 0) {
@@ -439,29 +480,41 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
                 ce = bad_y ? NAN : (log2f(s1) - xy) * LN2;
             }
             if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
-            else { a.row_kd[r] = term; a.row_ce[r] = ce; }
+            else { a.row_kd[r] = kd_on ? term : NO_TERM; a.row_ce[r] = ce_on ? ce : NO_TERM; }
         }
     }
-    if constexpr (NV > 0) {
+    if (dz) {
         const float ckd = bad ? NAN : kd_on ? g * a.kd * a.temp / s_cnt[0] : 0.f;
         const float cce = bad_y ? NAN : ce_on ? g * a.ce / s_cnt[1] : 0.f;
         const float akd = ckd / se, ace = cce / s1;          // (a term that the row does not have: 0)
-        int tid_again = tid;
-        asm volatile("" : "+v"(tid_again));                  // (the stores' offsets are made where they are used)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = i * NT + tid_again;
-            x[i].forget();
+        auto grad = [&](V& l, int c) {
+            l.forget();
             typename V::V o;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 float et, e1;
-                exps(x[i].get(e), mc, mc1, et, e1);
+                exps(l.get(e), mc, mc1, et, e1);
                 o[e] = ElemTraits<T>::from_float(SQ == 0 ? (akd + ace) * et : fmaf(ace, e1, akd * et));
             }
             V w;
             w.raw = __builtin_bit_cast(typename V::U, o);
-            if (c * N < vocab) w.store(dz, V::at(c, vocab));             // (where loads overlap, the same values twice)
+            if (c * N < vocab) w.store(dz, V::at(c, vocab));         // (where loads overlap, the same values twice)
+        };
+        int tid_again = tid;
+        asm volatile("" : "+v"(tid_again));              // (the stores' offsets are made where they are used)
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) grad(x[i], i * NT + tid_again);
+        } else {                                         // (a row too long for the registers: read a second time)
+            constexpr int DEEP = 4;
+            const int loads = (vocab + N - 1) / N;
+            for (int c0 = 0; c0 < loads; c0 += DEEP * NT) {
+                V l[DEEP];
+#pragma unroll
+                for (int i = 0; i < DEEP; ++i) l[i].load(z, V::at(c0 + i * NT + tid_again, vocab));
+#pragma unroll
+                for (int i = 0; i < DEEP; ++i) grad(l[i], c0 + i * NT + tid_again);
+            }
         }
         __syncthreads();                                     // the row's stores are done: its entries and the label are written again
         for (int j = tid; j <= top; j += NT) {
@@ -488,8 +541,10 @@ template <typename T, typename TV, int SQ>
 static void launch_rows(const DistillArgs& a, hipStream_t s) {
     const long long loads = ((long long)a.vocab + RowVec<T>::N - 1) / RowVec<T>::N;
 #define SUBREG_ROWS(NT, NV) hipLaunchKernelGGL((distill_row_kernel<T, TV, NT, NV, SQ>), a.rows, NT, 0, s, a)
-    if (a.vocab < RowVec<T>::N || loads <= 64 || (a.dz && loads > 1024 * 16)) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
-    else if (!a.dz) SUBREG_ROWS(256, 0);
+    if (a.vocab < RowVec<T>::N) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
+    else if (loads <= 64) SUBREG_ROWS(64, 1);
+    else if (loads <= 64 * 2) SUBREG_ROWS(64, 2);
+    else if (!a.dz || loads > 1024 * 16) SUBREG_ROWS(256, 0);
     else if (loads <= 256 * 4) SUBREG_ROWS(256, 4);
     else if (loads <= 256 * 8) SUBREG_ROWS(256, 8);
     else if (loads <= 256 * 16) SUBREG_ROWS(256, 16);
@@ -500,7 +555,7 @@ static void launch_rows(const DistillArgs& a, hipStream_t s) {
 
 template <typename TZ>
 static int distill_launch(const DistillArgs& a, int values_dtype, hipStream_t s) {
-    const bool count = a.reduction == SUBREG_MEAN && !(a.flags & SUBREG_DISTILL_COUNTED);
+    const bool count = a.reduction == SUBREG_MEAN && a.dz && a.count_blocks && !(a.flags & SUBREG_DISTILL_COUNTED);
     SUBREG_FOR_FLOAT(values_dtype, {
         if (count) hipLaunchKernelGGL(distill_count_kernel<T>, a.count_blocks, 256, 0, s, a);
         switch (a.target ? a.squarings : 0) {
@@ -540,6 +595,8 @@ extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     a.squarings = d->temperature == 1.f ? 0 : d->temperature == 2.f ? 1 : d->temperature == 4.f ? 2 : -1;
     a.count_rows = (int)((((long long)d->rows + COUNT_BLOCKS - 1) / COUNT_BLOCKS + 3) / 4 * 4);
     a.count_blocks = (int)(((long long)d->rows + a.count_rows - 1) / a.count_rows);
+    const int small = 128 * (16 / dtype_bytes(d->dtype));            // (the kernels for short rows know how)
+    if ((long long)d->rows * d->top <= COUNT_INLINE && d->vocab <= small) a.count_blocks = 0;
     a.temp = d->temperature; a.inv_t = 1.f / d->temperature; a.c_t = (float)(1.4426950408889634 / (double)d->temperature);
     a.kd = d->kd_weight; a.ce = d->ce_weight;
     a.gs = d->grad_scale; a.gs_stride = d->grad_scale_stride; a.loss = d->loss; a.dz = d->dlogits;

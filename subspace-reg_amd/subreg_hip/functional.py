@@ -240,10 +240,12 @@ def _rows(t, name):
 
 def _launch(dev, fn, what, *args):
     """fn(*args, stream) on the current stream of `dev`, with `dev` as the current device."""
-    if dev.index != torch.cuda.current_device():
+    if dev.index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            return _lib.check(fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), what)
-    return _lib.check(fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), what)
+            return _launch(dev, fn, what, *args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _ptr(t):
@@ -369,8 +371,7 @@ class DistillLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, tv, ti, target, need_grad, shape, *args):
         lib, dev = _lib.load(), z.device
-        nbytes = lib.subreg_distill_ws_bytes(z.shape[0])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.subreg_distill_ws_bytes(z.shape[0]), dtype=torch.uint8, device=dev)
         d = _distill_desc(z, tv, ti, target, *args, ws)
         loss = torch.empty(shape, dtype=torch.float32, device=dev)
         d.loss = loss.data_ptr()
@@ -378,26 +379,24 @@ class DistillLossFn(torch.autograd.Function):
             dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
             d.dlogits = dz.data_ptr()
             ctx.save_for_backward(z, tv, ti, target)
-            ctx.dz, ctx.ws, ctx.args = dz, ws, args
+            ctx.dz, ctx.ws, ctx.desc = dz, ws, d         # (the saved tensors and ws keep what the descriptor points at)
         _launch(dev, lib.subreg_distill_loss, "distill_loss", C.byref(d))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        z, tv, ti, target = ctx.saved_tensors
-        d = _distill_desc(z, tv, ti, target, *ctx.args, ctx.ws)
+        z, d, dz = ctx.saved_tensors[0], ctx.desc, ctx.dz
         g = g.reshape(-1)
         d.grad_scale, d.grad_scale_stride = g.data_ptr(), g.stride(0) if g.numel() > 1 else 0
-        d.flags = _lib.DISTILL_COUNTED
-        dz, ctx.dz = ctx.dz, None
-        if dz is None:                               # a second backward over a retained graph: the first took the buffer
-            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        d.loss = None
+        if dz is None:                                   # a second backward over a retained graph: the first took the buffer
+            d.flags, dz = _lib.DISTILL_COUNTED, torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            d.dlogits = dz.data_ptr()
         else:
-            d.flags |= _lib.DISTILL_SKIP_UNIT
-        d.dlogits = dz.data_ptr()
+            d.flags, ctx.dz = _lib.DISTILL_COUNTED | _lib.DISTILL_SKIP_UNIT, None
         _launch(z.device, _lib.load().subreg_distill_loss, "distill_loss(bwd)", C.byref(d))
-        return (dz,) + (None,) * (5 + len(ctx.args))
+        return dz, None, None, None, None, None, None, None, None, None, None
 
 
 def distill_loss(logits, top_values, top_indices, target=None, temperature=1.0, kd_weight=1.0, ce_weight=0.0, ignore_index=-100,
