@@ -85,11 +85,27 @@ __global__ __launch_bounds__(256) void quantize_any_rows_kernel(const T* __restr
         out[k] = k < dim ? (signed char)code_of(ElemTraits<T>::to_float(row[k]), inv) : 0;
 }
 
-// x given as codes: rows copied to the padded pitch
-__global__ __launch_bounds__(256) void pad_codes_kernel(const signed char* __restrict__ x, long long x_stride, int dim,
-                                                        signed char* __restrict__ codes, long long codes_stride) {
-    const long long r = blockIdx.x;
-    for (long long k = threadIdx.x; k < codes_stride; k += 256) codes[r * codes_stride + k] = k < dim ? x[r * x_stride + k] : 0;
+// codes copied to rows of the padded pitch (x given as codes, weights whose rows start anywhere): a thread per 16 bytes, which are read
+// at any address; the bytes of a row's last ones behind `dim`, and those that would be read past the last row, become 0
+__global__ __launch_bounds__(256) void pad_codes_kernel(const signed char* __restrict__ x, long long x_stride, int rows, int dim,
+                                                        signed char* __restrict__ codes, int pitch) {
+    const unsigned per = (unsigned)pitch / 16;
+    const unsigned long long id = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
+    const unsigned long long r = id / per;
+    if (r >= (unsigned long long)rows) return;
+    const int k = (int)(id - r * per) * 16, left = dim - k;          // left: bytes of the row from here
+    const signed char* from = x + (long long)r * x_stride;
+    i32x4 v = {0, 0, 0, 0};
+    if (left >= 16) {
+        __builtin_memcpy(&v, from + k, 16);
+    } else if (left > 0) {
+        unsigned long long lo = 0, hi = 0;
+#pragma unroll
+        for (int i = 0; i < 15; ++i)
+            if (i < left) (i < 8 ? lo : hi) |= (unsigned long long)(unsigned char)from[k + i] << (8 * (i & 7));
+        v = i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+    }
+    *(i32x4*)(codes + (long long)r * pitch + k) = v;
 }
 
 // 16 bytes of a weight row; bytes at or past `dim` come as zeros and are not read
@@ -297,6 +313,10 @@ __global__ __launch_bounds__(64 * W, 2) void linear_int8_rows_kernel(
 // Schedule of a stage (two k-steps): the reads of the second k-step run under the MFMAs of the first; the barrier stands in the MIDDLE
 // of the second k-step's MFMAs, and behind it the DMA of the stage after next and the reads of the next stage's first k-step run under
 // the other half.  A DMA has a whole stage of MFMAs to land.
+// 8192 x 4096 x 8192 takes 227 us (2.4 P operations a second; a large library product of 8-bit integers: 2.2).  What bounds it: the same
+// kernel without the DMA takes 186, without the fragment reads 214, without both and the barrier 169, of which 145 are the MFMAs - at 1.8
+// GHz, where the clock is 2.0 with everything on and 2.4 at rest: the costs add up, as power does.  Four stages of 64 bytes with three
+// in flight are slower (250), and so is any other place of the DMAs in the stage (228 - 240).
 // D = C + A B with C and D the same accumulator registers.  As an asm statement because hipcc (ROCm 7.2) gives the builtin's result
 // other registers than its addend and copies between them (376 copies beside the 128 MFMAs of a stage).  The operands come from LDS reads
 // (the compiler waits for those before the statement); before the results are read, mfma_done() lets the last one retire.
@@ -512,6 +532,11 @@ extern "C" int subreg_quantize_rows(const void* x, long long x_stride, int dtype
     return quantize(x, x_stride, dtype, rows, dim, codes, codes_stride, scale, (hipStream_t)stream);
 }
 
+static void pad_codes(const signed char* x, long long x_stride, int rows, int dim, signed char* codes, long long pitch, hipStream_t s) {
+    const unsigned long long blocks = ((unsigned long long)rows * (pitch / 16) + 255) / 256;
+    hipLaunchKernelGGL(pad_codes_kernel, (unsigned)blocks, 256, 0, s, x, x_stride, rows, dim, codes, (int)pitch);
+}
+
 // the weight as the tile kernel reads it: rows at multiples of 16 bytes, 32-bit offsets inside a tile
 static bool weight_direct(const signed char* w, long long w_stride) {
     return ((size_t)w & 15) == 0 && w_stride % 16 == 0 && w_stride <= (1 << 22);
@@ -573,7 +598,7 @@ extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype
     signed char* q = (signed char*)ws;
     float* s = (float*)(q + round_up(rows * pitch, 256));
     if (x_dtype == SUBREG_I8) {
-        hipLaunchKernelGGL(pad_codes_kernel, rows, 256, 0, st, (const signed char*)x, x_stride, dim, q, pitch);
+        pad_codes((const signed char*)x, x_stride, rows, dim, q, pitch, st);
     } else {
         const int rc = quantize(x, x_stride, x_dtype, rows, dim, q, pitch, s, st);
         if (rc) return rc;
@@ -606,14 +631,23 @@ extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype
     }
     if (!weight_direct(weight, w_stride)) {
         signed char* wp = (signed char*)s + round_up(4ll * rows, 256);
-        hipLaunchKernelGGL(pad_codes_kernel, out, 256, 0, st, weight, w_stride, dim, wp, pitch);
+        pad_codes(weight, w_stride, out, dim, wp, pitch, st);
         weight = wp;
         w_stride = pitch;
     }
-    const bool large = (long long)((rows + 255) / 256) * ((out + 255) / 256) >= 200;
+    // Tiles.  256 x 256 (a block a CU) does a tile's work in 1 / 1.2 of the time of four 128 x 128 ones, but in whole rounds of the 256 CUs:
+    // us, 256 | 128: 8192 x 4096 x 4096 128 | 161; 3000 x 4096 x 5000 (240 tiles, one round) 70 | 73; 5000 x 2048 x 5000 (400, two) 81 | 75.
+    // Where 128 x 128 makes 256 tiles or fewer, 64 x 128, and 64 x 64 where those do not fill the chip (128 | 64 x 128 | 64 x 64:
+    // 2048 x 4096 x 2048 32.8 | 30.9 | 36.0; 1024 x 1024 x 4096 13.4 | 12.7 | 13.3; 333 x 1111 x 5003 22.0 | 19.5 | 19.0;
+    // 128 x 4096 x 4096 26.0 | 23.1 | 20.3).
+    auto tiles = [&](int tm, int tn) { return (long long)((rows + tm - 1) / tm) * ((out + tn - 1) / tn); };
+    const long long n128 = tiles(128, 128);
     SUBREG_FOR_FLOAT(y_dtype, {
-        if (large) return launch_tiles<8, 8, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
-        return launch_tiles<4, 4, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+        if (20 * ((tiles(256, 256) + 255) / 256 * 256) <= 6 * n128)
+            return launch_tiles<8, 8, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+        if (n128 > 256) return launch_tiles<4, 4, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+        if (tiles(64, 128) >= 256) return launch_tiles<2, 4, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
+        return launch_tiles<2, 2, T>(q, (int)pitch, sx, weight, (int)w_stride, w_scale, bias, y, rows, dim, out, st);
     })
     return SUBREG_EINVAL;
 }

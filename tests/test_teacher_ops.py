@@ -241,8 +241,9 @@ def test_quantize_rows_extremes_and_shapes():
     assert HF.quantize_rows(torch.zeros(0, 5).cuda())[0].shape == (0, 5)
 
 
-LINEAR = [(1, 1, 1), (1, 640, 351), (2, 64, 16), (3, 4096, 1000), (5, 17, 33), (16, 128, 64), (17, 129, 65), (33, 1111, 130),
-          (48, 2048, 257), (64, 640, 351), (100, 96, 700), (129, 512, 129), (257, 384, 300), (300, 1000, 520), (520, 272, 1030)]
+LINEAR = [(1, 1, 1), (1, 640, 351), (2, 64, 16), (3, 4096, 1000), (5, 17, 33), (16, 128, 64), (17, 129, 65), (33, 1111, 130), (1, 20, 100), (1, 2047, 700), (1, 5000, 90), (1, 9000, 50), (30, 200, 9000), (40, 300, 17000), (60, 100, 16500),
+          (48, 2048, 257), (64, 640, 351), (100, 96, 700), (129, 512, 129), (257, 384, 300), (300, 1000, 520), (520, 272, 1030),
+          (1100, 200, 2100), (2100, 130, 2050), (2600, 65, 5200)]
 
 
 def check_linear(x, w, ws, bias, got, out_dtype, codes=None):
