@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256) void distill_any_kernel(DistillArgs a) {
 // NT threads per row, NV loads of 16 bytes a thread in registers; NV = 0: the row streamed with a running maximum and sum a thread (few
 // registers, any length): the loss alone, and rows that do not fit the registers, which are then read a second time.  SQ: squarings from e to e1 (-1: a second exponential; 0: T = 1, or no
 // labels).  The first wave does the teacher's side while the others' loads are in flight.
-template <typename T, typename TV, int NT, int NV, int SQ>
+template <typename T, typename TV, int NT, int NV, int SQ, bool STREAM = false>
 __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     using V = RowVec<T>;
     constexpr int N = V::N, EPL = SUBREG_TOP_MAX / 64;              // entries a lane
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     }
     V x[NV ? NV : 1];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i].load(z, V::at(i * NT + tid, vocab));
+    for (int i = 0; i < NV; ++i) x[i].template load_as<STREAM>(z, V::at(i * NT + tid, vocab));
 
     // the teacher's shares (first wave) and the counts (last wave)
     float p[EPL], tm = -INFINITY, ps = 0.f, z_at[EPL], z_y = 0.f;
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
             }
             V w;
             w.raw = __builtin_bit_cast(typename V::U, o);
-            if (c * N < vocab) w.store(dz, V::at(c, vocab));         // (where loads overlap, the same values twice)
+            if (c * N < vocab) w.template store_as<STREAM>(dz, V::at(c, vocab));   // (where loads overlap, the same values twice)
         };
         int tid_again = tid;
         asm volatile("" : "+v"(tid_again));              // (the stores' offsets are made where they are used)
@@ -540,17 +540,34 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
 template <typename T, typename TV, int SQ>
 static void launch_rows(const DistillArgs& a, hipStream_t s) {
     const long long loads = ((long long)a.vocab + RowVec<T>::N - 1) / RowVec<T>::N;
+    // logits and gradient that the last-level cache (256 MB) does not hold together go past it: 4096 x 32000 bf16 140 -> 121 us a call,
+    // 1024 x 131072 162 -> 152; 512 x 32000, which it holds, 30.6 -> 29.8
+    const bool stream = (long long)a.rows * a.vocab * (long long)sizeof(T) >= (128ll << 20);
+#define SUBREG_STREAM(NT, NV)                                                                                       \
+    if (stream) hipLaunchKernelGGL((distill_row_kernel<T, TV, NT, NV, SQ, true>), a.rows, NT, 0, s, a);             \
+    else SUBREG_ROWS(NT, NV)
 #define SUBREG_ROWS(NT, NV) hipLaunchKernelGGL((distill_row_kernel<T, TV, NT, NV, SQ>), a.rows, NT, 0, s, a)
-    if (a.vocab < RowVec<T>::N) hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
-    else if (loads <= 64) SUBREG_ROWS(64, 1);
-    else if (loads <= 64 * 2) SUBREG_ROWS(64, 2);
-    else if (!a.dz || loads > 1024 * 16) SUBREG_ROWS(256, 0);
-    else if (loads <= 256 * 4) SUBREG_ROWS(256, 4);
-    else if (loads <= 256 * 8) SUBREG_ROWS(256, 8);
-    else if (loads <= 256 * 16) SUBREG_ROWS(256, 16);
-    else if (loads <= 512 * 16) SUBREG_ROWS(512, 16);
-    else SUBREG_ROWS(1024, 16);
+    if (a.vocab < RowVec<T>::N) {
+        hipLaunchKernelGGL((distill_any_kernel<T, TV>), a.rows, 256, 0, s, a);
+    } else if (loads <= 64) {
+        SUBREG_ROWS(64, 1);
+    } else if (loads <= 64 * 2) {
+        SUBREG_ROWS(64, 2);
+    } else if (!a.dz || loads > 1024 * 16) {
+        SUBREG_ROWS(256, 0);
+    } else if (loads <= 256 * 4) {
+        SUBREG_ROWS(256, 4);
+    } else if (loads <= 256 * 8) {
+        SUBREG_ROWS(256, 8);
+    } else if (loads <= 256 * 16) {
+        SUBREG_STREAM(256, 16);
+    } else if (loads <= 512 * 16) {
+        SUBREG_STREAM(512, 16);
+    } else {
+        SUBREG_STREAM(1024, 16);
+    }
 #undef SUBREG_ROWS
+#undef SUBREG_STREAM
 }
 
 template <typename TZ>

@@ -57,6 +57,16 @@ template <typename T> struct RowVec {
     __device__ __forceinline__ void store(T* row, int at) const { __builtin_memcpy((char*)row + bytes(at), &raw, 16); }
     __device__ __forceinline__ T elem(int e) const { return __builtin_bit_cast(V, raw)[e]; }
     __device__ __forceinline__ float get(int e) const { return ElemTraits<T>::to_float(elem(e)); }
+    // past the caches (STREAM), for matrices that no cache holds until their next reader
+    typedef U __attribute__((aligned(1))) UA;
+    template <bool STREAM> __device__ __forceinline__ void load_as(const T* row, int at) {
+        if constexpr (STREAM) raw = __builtin_nontemporal_load((const UA*)((const char*)row + bytes(at)));
+        else load(row, at);
+    }
+    template <bool STREAM> __device__ __forceinline__ void store_as(T* row, int at) const {
+        if constexpr (STREAM) __builtin_nontemporal_store(raw, (UA*)((char*)row + bytes(at)));
+        else store(row, at);
+    }
     // between two uses of a held row: what the first use unpacked is unpacked again (kept, it would take twice the registers)
     __device__ __forceinline__ void forget() { asm volatile("" : "+v"(raw)); }
 };

@@ -241,7 +241,8 @@ def test_quantize_rows_extremes_and_shapes():
     assert HF.quantize_rows(torch.zeros(0, 5).cuda())[0].shape == (0, 5)
 
 
-LINEAR = [(1, 1, 1), (1, 640, 351), (2, 64, 16), (3, 4096, 1000), (5, 17, 33), (16, 128, 64), (17, 129, 65), (33, 1111, 130), (1, 20, 100), (1, 2047, 700), (1, 5000, 90), (1, 9000, 50), (30, 200, 9000), (40, 300, 17000), (60, 100, 16500),
+LINEAR = [(1, 1, 1), (1, 640, 351), (2, 64, 16), (3, 4096, 1000), (5, 17, 33), (16, 128, 64), (17, 129, 65), (33, 1111, 130),
+          (1, 20, 100), (1, 2047, 700), (1, 5000, 90), (1, 9000, 50), (30, 200, 9000), (40, 300, 17000), (60, 100, 16500),
           (48, 2048, 257), (64, 640, 351), (100, 96, 700), (129, 512, 129), (257, 384, 300), (300, 1000, 520), (520, 272, 1030),
           (1100, 200, 2100), (2100, 130, 2050), (2600, 65, 5200)]
 
@@ -479,6 +480,35 @@ def test_distill_masks_and_bad_entries(v, dtype):
     loss = HF.distill_loss(leaf, tv[:1], ti[:1], None, 2.0)
     loss.backward()
     assert loss.item() == math.inf and torch.isfinite(leaf.grad).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,v,dtype", [(2100, 32003, torch.bfloat16), (1150, 60000, torch.float16), (530, 131072, torch.bfloat16),
+                                       (2100, 16001, torch.float32)])
+def test_distill_large_matrices_row_by_row(n, v, dtype):
+    """Matrices that go past the caches (128 MB and more): every row's loss and gradient is that of a call on fewer rows, bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    z = torch.randn(n, v, generator=g, device="cuda").mul_(2.5).to(dtype)
+    tv, ti = torch.topk(z[:, 7:1000].float(), 30, dim=1)
+    y = torch.randint(0, v, (n,), generator=g, device="cuda")
+    y[3] = -100
+    ti[3] = -1
+
+    def run(rows):
+        leaf = z[rows].detach().requires_grad_()
+        loss = HF.distill_loss(leaf, tv[rows].to(dtype), ti[rows], y[rows], 2.0, 0.5, 0.5, reduction="none")
+        loss.sum().backward()
+        return loss.detach(), leaf.grad
+
+    loss, grad = run(slice(0, n))
+    for lo in range(0, n, n // 3):
+        part = run(slice(lo, lo + n // 3))
+        assert torch.equal(part[0], loss[lo:lo + n // 3]) and torch.equal(part[1], grad[lo:lo + n // 3])
+    rows = [0, 3, n // 2, n - 1]
+    want, wg = plain_distill(z[rows], tv[rows].to(dtype), ti[rows], y[rows], 2.0, 0.5, 0.5, reduction="none")
+    row, elem = distill_bounds(z[rows], tv[rows], ti[rows], 2.0, 0.5, 0.5)
+    close(loss[rows], want, row)
+    close(grad[rows], wg, elem, dtype)
 
 
 @gpu
