@@ -449,7 +449,8 @@ int subreg_validate(const float* feat, const long long* labels, const float* wei
 /* ---- teacher / student operators: the 8-bit linear head, a row's largest logits, the distillation loss -----------------------
  * (what the reference's distill/ holds losses for: the answers of a frozen teacher and a student that is trained on them.)
  * dtype / x_dtype / y_dtype: SUBREG_F32 | SUBREG_BF16 | SUBREG_F16.  Rows are contiguous; `*_stride` is the distance of two rows in
- * ELEMENTS (0 allowed for inputs: one row seen many times).  Up to 2^30 columns; offsets are 64-bit.  Sums and softmax statistics are fp32 or wider.
+ * ELEMENTS (0 allowed for inputs: one row seen many times).  Up to 2^22 - 1 rows and 2^30
+ * columns a call; offsets are 64-bit.  Sums and softmax statistics are fp32 or wider.
  * `ws`: scratch of the size the matching subreg_*_ws_bytes returns, 256-byte aligned, used by this call alone while it runs. */
 
 /* Codes of each row x[r][0..dim): a = max(max_k |x|, 2^-100), scale[r] = a / 127, code = rint(x * (127 / a)) in [-127, 127], where both
@@ -462,7 +463,7 @@ int subreg_quantize_rows(const void* x, long long x_stride, int dtype, int rows,
  * SUBREG_I8_MAX_DIM), one rounding to y_dtype.  x_dtype SUBREG_I8: q = x, s = x_scale.  Otherwise q, s are what subreg_quantize_rows
  * makes of x, within the call.  y is [rows][out], contiguous.
  * weight rows: where w_stride and the address are multiples of 16, bytes dim .. round_up(dim, 16) of each row must be readable (their
- * values do not matter); the same holds for x of SUBREG_I8. */
+ * values do not matter).  The size of ws follows from the weight's address and stride: pass the ones of the call. */
 #define SUBREG_I8_MAX_DIM 131071
 long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype, const signed char* weight, long long w_stride);
 int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const float* x_scale, const signed char* weight,

@@ -593,13 +593,13 @@ using namespace subreg;
 static inline long long distill_align(long long b) { return (b + 255) / 256 * 256; }
 
 extern "C" long long subreg_distill_ws_bytes(int rows) {
-    if (rows <= 0) return SUBREG_EINVAL;
+    if (rows <= 0 || rows > MAX_ROWS) return SUBREG_EINVAL;
     return 2 * distill_align(4ll * rows) + distill_align(8 * COUNT_BLOCKS);
 }
 
 extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     SUBREG_CHECK_ARG(d && d->logits && d->top_values && d->top_indices && (d->loss || d->dlogits));
-    SUBREG_CHECK_ARG(d->rows > 0 && d->vocab > 0 && d->vocab <= MAX_COLUMNS && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
+    SUBREG_CHECK_ARG(d->rows > 0 && d->rows <= MAX_ROWS && d->vocab > 0 && d->vocab <= MAX_COLUMNS && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
     SUBREG_CHECK_ARG(d->logits_stride >= 0 && d->values_stride >= 0 && d->indices_stride >= 0 && d->grad_scale_stride >= 0);
     SUBREG_CHECK_ARG(float_dtype(d->dtype) && float_dtype(d->values_dtype) && d->temperature > 0.f && d->temperature <= 3.0e38f);
     SUBREG_CHECK_ARG(d->reduction >= SUBREG_NONE && d->reduction <= SUBREG_MEAN);

@@ -528,7 +528,7 @@ using namespace subreg;
 
 extern "C" int subreg_quantize_rows(const void* x, long long x_stride, int dtype, int rows, int dim, signed char* codes,
                                     long long codes_stride, float* scale, void* stream) {
-    SUBREG_CHECK_ARG(x && codes && scale && rows > 0 && dim > 0 && dim <= MAX_COLUMNS && x_stride >= 0 && codes_stride >= dim && float_dtype(dtype));
+    SUBREG_CHECK_ARG(x && codes && scale && rows > 0 && rows <= MAX_ROWS && dim > 0 && dim <= MAX_COLUMNS && x_stride >= 0 && codes_stride >= dim && float_dtype(dtype));
     return quantize(x, x_stride, dtype, rows, dim, codes, codes_stride, scale, (hipStream_t)stream);
 }
 
@@ -543,7 +543,7 @@ static bool weight_direct(const signed char* w, long long w_stride) {
 }
 
 extern "C" long long subreg_linear_int8_ws_bytes(int rows, int dim, int out, int x_dtype, const signed char* weight, long long w_stride) {
-    if (rows <= 0 || dim <= 0 || dim > SUBREG_I8_MAX_DIM || out <= 0 || w_stride < 0 || !(float_dtype(x_dtype) || x_dtype == SUBREG_I8))
+    if (rows <= 0 || rows > MAX_ROWS || dim <= 0 || dim > SUBREG_I8_MAX_DIM || out <= 0 || out > MAX_ROWS || w_stride < 0 || !(float_dtype(x_dtype) || x_dtype == SUBREG_I8))
         return SUBREG_EINVAL;
     const long long pitch = round_up(dim, I8_PITCH);
     return round_up(rows * pitch, 256) + round_up(4ll * rows, 256) + (rows <= ROWS_MOST || weight_direct(weight, w_stride) ? 0 : round_up(out * pitch, 256));
@@ -558,7 +558,7 @@ static int launch_tiles(const signed char* q, int pitch, const float* s, const s
     const int rc = ensure_dynamic_lds((const void*)kern, S::LDS, ready);
     if (rc) return rc;
     const long long tiles = (long long)((rows + S::TM - 1) / S::TM) * ((out + S::TN - 1) / S::TN);
-    if (tiles > 0x7fffffff) return SUBREG_EUNSUPPORTED;
+    if (tiles >= 1ll << 24) return SUBREG_EUNSUPPORTED;             // (a grid of 2^32 threads)
     hipLaunchKernelGGL(kern, (unsigned)tiles, 256, S::LDS, st, q, pitch, s, w, w_stride, t, bias, (T*)y, rows, dim, out);
     return launch_status();
 }
@@ -589,7 +589,8 @@ static int launch_gemv(const signed char* q, const float* sx, const signed char*
 extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype, const float* x_scale, const signed char* weight,
                                   long long w_stride, const float* w_scale, const float* bias, void* y, int y_dtype, int rows,
                                   int dim, int out, void* ws, long long ws_bytes, void* stream) {
-    SUBREG_CHECK_ARG(x && weight && w_scale && y && ws && rows > 0 && dim > 0 && dim <= SUBREG_I8_MAX_DIM && out > 0);
+    SUBREG_CHECK_ARG(x && weight && w_scale && y && ws && rows > 0 && rows <= MAX_ROWS && dim > 0 && dim <= SUBREG_I8_MAX_DIM);
+    SUBREG_CHECK_ARG(out > 0 && out <= MAX_ROWS);
     SUBREG_CHECK_ARG(x_stride >= 0 && w_stride >= 0 && float_dtype(y_dtype) && (float_dtype(x_dtype) || x_dtype == SUBREG_I8));
     SUBREG_CHECK_ARG((x_dtype == SUBREG_I8) == (x_scale != nullptr) && ((size_t)ws & 255) == 0);
     SUBREG_CHECK_ARG(ws_bytes >= subreg_linear_int8_ws_bytes(rows, dim, out, x_dtype, weight, w_stride));
@@ -604,7 +605,7 @@ extern "C" int subreg_linear_int8(const void* x, long long x_stride, int x_dtype
         if (rc) return rc;
     }
     const float* sx = x_dtype == SUBREG_I8 ? x_scale : s;
-    if (rows == 1 && dim >= 16 && dim <= GEMV_MOST && out < 0x7fff0000) {       // (out: the waves' channel numbers stay inside 32 bits)
+    if (rows == 1 && dim >= 16 && dim <= GEMV_MOST) {
         SUBREG_FOR_FLOAT(y_dtype, {
             if (dim <= 1024) return (launch_gemv<T, 1, 8>(q, sx, weight, w_stride, w_scale, bias, (T*)y, dim, out, st));
             if (dim <= 2048) return (launch_gemv<T, 2, 8>(q, sx, weight, w_stride, w_scale, bias, (T*)y, dim, out, st));

@@ -11,6 +11,7 @@ template <> struct ElemTraits<_Float16> {
 };
 
 constexpr int MAX_COLUMNS = 1 << 30;      // of a row: column arithmetic stays inside 32 bits
+constexpr int MAX_ROWS = (1 << 22) - 1;   // of a call: a grid has fewer than 2^32 threads, and a row up to 1024 of them
 
 inline bool float_dtype(int dt) { return dt == SUBREG_F32 || dt == SUBREG_BF16 || dt == SUBREG_F16; }
 inline int dtype_bytes(int dt) { return dt == SUBREG_F32 ? 4 : dt == SUBREG_I8 ? 1 : 2; }

@@ -359,7 +359,7 @@ using namespace subreg;
 
 extern "C" int subreg_top_logits(const void* logits, long long stride, int dtype, int rows, int vocab, int top, void* values,
                                  long long* indices, void* stream) {
-    SUBREG_CHECK_ARG(logits && values && indices && rows > 0 && vocab > 0 && vocab <= MAX_COLUMNS && stride >= 0);
+    SUBREG_CHECK_ARG(logits && values && indices && rows > 0 && rows <= MAX_ROWS && vocab > 0 && vocab <= MAX_COLUMNS && stride >= 0);
     SUBREG_CHECK_ARG(top >= 1 && top <= vocab && top <= SUBREG_TOP_MAX);
     SUBREG_FOR_FLOAT(dtype, return launch_top<T>((const T*)logits, stride, rows, vocab, top, (T*)values, indices, (hipStream_t)stream))
     return SUBREG_EINVAL;

@@ -233,8 +233,8 @@ def _rows(t, name):
         raise ValueError("%s needs a last dimension of at least one element, got shape %s" % (name, tuple(t.shape)))
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] > 2 ** 31 - 1 or t.shape[1] > 2 ** 30:
-        raise ValueError("%s: more than 2^31 - 1 rows or 2^30 columns" % name)
+    if t.shape[0] >= 2 ** 22 or t.shape[1] > 2 ** 30:
+        raise ValueError("%s: %d rows of %d; a call takes up to 2^22 - 1 rows of up to 2^30" % (name, t.shape[0], t.shape[1]))
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -314,8 +314,6 @@ def linear_int8(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
     dev = _on_device(x=x, weight=weight, weight_scale=weight_scale, bias=bias, x_scale=x_scale)
     if not _readable16(w):
         w = torch.nn.functional.pad(w, (0, -dim % 16))[:, :dim]
-    if code == _lib.I8 and not _readable16(rows):
-        rows = torch.nn.functional.pad(rows, (0, -dim % 16))[:, :dim]
     m = rows.shape[0]
     y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
     if m:

@@ -160,6 +160,11 @@ def test_refusals_on_cpu():
         HF.top_logits(f(2, 8, dtype=torch.int32), 1)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         HF.top_logits(f(2, 8), 1)
+    many = f(1, 8).expand(1 << 22, 8)
+    for call in (lambda: HF.quantize_rows(many), lambda: HF.top_logits(many, 1), lambda: HF.linear_int8(many, w, s),
+                 lambda: HF.linear_int8(f(1, 8), w[:1].expand(1 << 22, 8), s[:1].expand(1 << 22))):
+        with pytest.raises(ValueError, match="rows"):
+            call()
     i = f(2, 3, dtype=torch.int64)
     good = dict(logits=f(2, 8), top_values=f(2, 3), top_indices=i)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
@@ -181,17 +186,18 @@ def test_c_entries_refuse_on_cpu():
     assert lib.subreg_quantize_rows(None, 8, 0, 1, 8, p, 16, p, None) == -1
     assert lib.subreg_quantize_rows(p, 8, 0, 1, 8, p, 7, p, None) == -1
     assert lib.subreg_quantize_rows(p, 8, 3, 1, 8, p, 16, p, None) == -1
+    assert lib.subreg_quantize_rows(p, 8, 0, 1 << 22, 8, p, 16, p, None) == -1
     n = lib.subreg_linear_int8_ws_bytes(4, 100, 7, 0, p, 100)
     assert n >= 4 * 100 and lib.subreg_linear_int8_ws_bytes(4, _lib.I8_MAX_DIM + 1, 7, 0, p, 100) == -1
     args = [p, 100, 0, None, p, 100, p, None, p, 0, 4, 100, 7, p, n, None]
-    for at, value in ((0, None), (2, 3), (2, 9), (3, p), (9, 3), (10, 0), (11, 0), (11, _lib.I8_MAX_DIM + 1), (12, 0), (13, None), (13, p + 8),
+    for at, value in ((0, None), (2, 3), (2, 9), (3, p), (9, 3), (10, 0), (11, 0), (11, _lib.I8_MAX_DIM + 1), (12, 0), (12, 1 << 22), (10, 1 << 22), (13, None), (13, p + 8),
                       (14, n - 1), (5, -1)):
         bad = list(args)
         bad[at] = value
         assert lib.subreg_linear_int8(*bad) == -1, at
     for bad in ((None, 8, 0, 1, 8, 1, p, p, None), (p, 8, 0, 1, 8, 9, p, p, None), (p, 300, 0, 1, 300, 257, p, p, None),
                 (p, 8, 3, 1, 8, 1, p, p, None), (p, -1, 0, 1, 8, 1, p, p, None), (p, 8, 0, 0, 8, 1, p, p, None),
-                (p, 8, 0, 1, (1 << 30) + 1, 1, p, p, None)):
+                (p, 8, 0, 1, (1 << 30) + 1, 1, p, p, None), (p, 8, 0, 1 << 22, 8, 1, p, p, None)):
         assert lib.subreg_top_logits(*bad) == -1
     assert lib.subreg_distill_ws_bytes(0) == -1
 
@@ -204,7 +210,7 @@ def test_c_entries_refuse_on_cpu():
             setattr(d, k, v)
         return ctypes.byref(d)
 
-    for bad in (dict(logits=None), dict(top_values=None), dict(top_indices=None), dict(loss=None), dict(rows=0), dict(vocab=0), dict(top=0),
+    for bad in (dict(logits=None), dict(top_values=None), dict(top_indices=None), dict(loss=None), dict(rows=0), dict(rows=1 << 22), dict(vocab=0), dict(top=0),
                 dict(top=257), dict(temperature=0.0), dict(temperature=math.nan), dict(dtype=3), dict(values_dtype=3), dict(reduction=3),
                 dict(ws=None), dict(ws=p + 4), dict(ws_bytes=8), dict(flags=1), dict(logits_stride=-1)):
         assert lib.subreg_distill_loss(desc(**bad), None) == -1, bad
