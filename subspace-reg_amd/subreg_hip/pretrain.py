@@ -82,15 +82,24 @@ class GradientSync:
         import torch.distributed as dist
         self.dist, self.group = dist, group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
+        # gloo (tests, several ranks on one GPU) gets host tensors: a synchronous copy out, the result back in finish()
+        self.host_staged = dist.is_initialized() and dist.get_backend(group) == "gloo"
         self.calls = 0
-        self.pending, self.covered = [], []
+        self.pending, self.covered, self.staged = [], [], []
+
+    def _reduce(self, t):
+        if self.host_staged and t.is_cuda:
+            host = t.cpu()
+            self.staged.append((t, host))
+            t = host
+        self.pending.append(self.dist.all_reduce(t, op=self.dist.ReduceOp.SUM, group=self.group, async_op=True))
+        self.calls += 1
 
     def stage_ready(self, flat_slice):
         if self.world == 1:
             return
-        self.pending.append(self.dist.all_reduce(flat_slice, op=self.dist.ReduceOp.SUM, group=self.group, async_op=True))
+        self._reduce(flat_slice)
         self.covered.append((flat_slice.data_ptr(), flat_slice.data_ptr() + flat_slice.numel() * flat_slice.element_size()))
-        self.calls += 1
 
     def finish(self, params):
         if self.world == 1:
@@ -108,13 +117,14 @@ class GradientSync:
         for key, (base, views) in todo.items():
             # a storage none of whose views went out with a stage: ONE collective for the whole storage; otherwise view by view
             for t in ([base] if key not in partly else [v.contiguous() if not v.is_contiguous() else v for v in views]):
-                self.pending.append(self.dist.all_reduce(t, op=self.dist.ReduceOp.SUM, group=self.group, async_op=True))
-                self.calls += 1
+                self._reduce(t)
         try:
             for w in self.pending:
                 w.wait()
+            for t, host in self.staged:
+                t.copy_(host)
         finally:                                                # never carry handles / ranges of a failed step into the next
-            self.pending, self.covered = [], []
+            self.pending, self.covered, self.staged = [], [], []
 
     __call__ = finish
 
@@ -310,7 +320,7 @@ def fit(model, opt, train_loader, val_loader=None, lang_puller=None, rank=0, wor
     finally:
         if sync is not None:                                    # a backward outside fit() must not start collectives nobody waits on
             model.hip_backbone().grad_stage_hook = None
-            sync.pending, sync.covered = [], []
+            sync.pending, sync.covered, sync.staged = [], [], []
     if rank == 0:                                                                                 # :193-202
         ck.save_checkpoint(os.path.join(opt.model_path, "{}_last.pth".format(opt.model)), model, opt=opt,
                            **_continual_extra(opt, train_loader))
