@@ -584,6 +584,34 @@ def test_distill_gradient_against_differences():
     assert abs((ends[0] - ends[1]) / (2 * h) - slope) <= bound
 
 
+# ------------------------------------------------------------------------------------------------ far rows
+@gpu
+def test_rows_behind_the_32_bit_offsets():
+    """Logits, gradients and products of more than 2^32 bytes: the last rows are those of a call on them alone, bit for bit."""
+    n, v = 70001, 32000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.empty(n, v, device="cuda", dtype=torch.bfloat16)
+    z[:1000].normal_(generator=g)
+    for lo in range(1000, n, 1000):
+        z[lo:lo + 1000] = z[lo - 1000:lo][: min(1000, n - lo)]
+    z[-40:].normal_(generator=g)
+    tv, ti = torch.topk(z[:, :64].float(), 5, dim=1)
+    last = slice(n - 40, n)
+    values, indices = HF.top_logits(z, 7)
+    few = HF.top_logits(z[last].clone(), 7)
+    assert torch.equal(values[last], few[0]) and torch.equal(indices[last], few[1])
+    grads = []
+    for rows in (slice(0, n), last):
+        leaf = z[rows].detach().requires_grad_()
+        HF.distill_loss(leaf, tv[rows], ti[rows], None, 2.0, reduction="sum").backward()
+        grads.append(leaf.grad[-40:].clone())
+        del leaf
+    assert torch.equal(*grads)
+    x = rnd((n, 16), 3, torch.bfloat16)
+    w, ws = HF.quantize_rows(rnd((v, 16), 4))
+    assert torch.equal(HF.linear_int8(x, w, ws)[last], HF.linear_int8(x[last], w, ws))
+
+
 # ------------------------------------------------------------------------------------------------ together
 @gpu
 def test_results_do_not_change_from_call_to_call():
