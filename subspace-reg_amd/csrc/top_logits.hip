@@ -39,7 +39,7 @@ template <> struct TopKey<_Float16> : TopKey16<_Float16, 0x7c00u> {};
 //      loads where two of them reach t), and logits with a key >= t are listed in LDS; each takes the place that the count of larger (key, lower index) pairs gives it.
 // More than CAP candidates (ties, masked rows): select_exact.
 // Nothing of the row is held: at 64 registers a thread eight blocks of 256 share a CU, and the chain 2 - 3 of some (5 us) runs under the
-// reads of others.  With the row in registers (512 threads, 8 loads each, four blocks a CU in step) 2048 rows of 32000 took 40 us.
+// reads of others: 2048 rows of 32000 bf16 in 27 us, 4.9 TB/s, what a large copy reaches.  With the row in registers (512 threads, 8 loads each, four blocks a CU in step) they took 40.
 constexpr int CAP = 1024;
 constexpr int TOP_SHORT = 512;
 

@@ -406,7 +406,8 @@ def distill_loss(logits, top_values, top_indices, target=None, temperature=1.0, 
         kd_weight T^2 KL(softmax(top_values / T) || softmax(logits / T)) + ce_weight CE(logits, target)
     with the teacher's softmax over the row's kept entries.  A row without kept entries has no first term, one whose target is
     ignore_index no second; a row with neither is not read, its gradient is 0.  reduction "mean": each term over the rows that have it
-    (no such row: 0); "sum"; "none": [...].  Gradient for the logits only, in their type.  An index >= V, or a target outside
+    (no such row: 0); "sum"; "none": [...].  Gradient for the logits only, in their type;
+    inside a captured graph take it with torch.autograd.grad (as train.GraphedStep does), not with backward().  An index >= V, or a target outside
     [0, V), makes its row's loss and gradient NaN."""
     _float_code(logits, "logits")
     _float_code(top_values, "top_values")

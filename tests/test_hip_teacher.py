@@ -489,6 +489,37 @@ def test_distill_masks_and_bad_entries(v, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("v", [300, 3001, 50021, 140003])
+@pytest.mark.parametrize("temp", [1.0, 2.0, 3.0, 0.01])
+def test_distill_numbers_as_masks_and_far_logits(v, dtype, temp):
+    """Masks that are large numbers, in part of a row (whole threads see nothing else) and in all of it; logits far from 0."""
+    masks = [-1e4, -1e6, -3e7, -1e9, -1e10, -1e20, -1e30, torch.finfo(dtype).min]
+    z = rnd((2 * len(masks) + 6, v), 3, dtype, 2.5)
+    for i, m in enumerate(masks):
+        z[2 * i, 40:] = m
+        z[2 * i + 1] = m
+    for i, far in enumerate((1e4, -1e4, 1e6, -1e6, 1e8, -1e8)):
+        z[2 * len(masks) + i] = (z[2 * len(masks) + i].float() + far).to(dtype)
+    n = z.shape[0]
+    ti = torch.arange(30, 38).expand(n, 8).clone().cuda()
+    tv = rnd((n, 8), 4, dtype)
+    y = torch.arange(n).cuda()
+    near = torch.where(z < z.max(1, keepdim=True).values - 200, z.max(1, keepdim=True).values, z)    # (masked logits carry no share)
+    row, elem = distill_bounds(near, tv, ti, temp, 0.5, 0.5)
+    for reduction in ("none", "mean"):
+        leaf = z.detach().requires_grad_()
+        loss = HF.distill_loss(leaf, tv, ti, y, temp, 0.5, 0.5, reduction=reduction)
+        loss.sum().backward()
+        want, grad = plain_distill(z, tv, ti, y, temp, 0.5, 0.5, reduction=reduction)
+        close(loss.detach().reshape(-1), want.reshape(-1), 2 * row, note="loss")
+        close(leaf.grad, grad, elem, dtype, "gradient")
+        with torch.no_grad():
+            alone = HF.distill_loss(leaf, tv, ti, y, temp, 0.5, 0.5, reduction=reduction)
+        close(alone.reshape(-1), want.reshape(-1), 2 * row, note="the loss alone")
+
+
+@gpu
 @pytest.mark.parametrize("n,v,dtype", [(2100, 32003, torch.bfloat16), (1150, 60000, torch.float16), (530, 131072, torch.bfloat16),
                                        (2100, 16001, torch.float32)])
 def test_distill_large_matrices_row_by_row(n, v, dtype):
