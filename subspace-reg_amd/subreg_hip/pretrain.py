@@ -157,19 +157,24 @@ def _batch_metrics(output, target, counters):
     return loss, 100.0 * c[0] / n, 100.0 * c[1] / n
 
 
+def _classes(model):
+    """Rows of the classifier (num_classes stays behind when classes are added, as in the reference)."""
+    return model.classifier.weight.shape[0] if model.num_classes > 0 else 0
+
+
 class Teacher:
     """A frozen network as a teacher: `teacher(images)` -> (values [B, top], indices [B, top]), its `top` largest logits per image.
 
     int8_head: the classifier's product in 8 bits (functional.linear_int8: codes and scales of the weight are made here, once; the
     features are quantised per image).  Train a student on it with `train(..., teacher=)` / `fit(..., teacher=)`: the loss is
     functional.distill_loss with opt.distill_temperature (4), opt.distill_weight (0.5) and opt.distill_ce_weight (0.5).
-    The network is put in eval mode and its weights are taken as they are now."""
+    The network is put in eval mode; an 8-bit head holds the classifier's weights as they are now."""
 
     def __init__(self, model, top=10, int8_head=False):
         self.model = model.eval()
-        self.top = int(top)
-        if not 1 <= self.top <= min(model.num_classes, HF._lib.TOP_MAX):
-            raise ValueError("top = %d of a teacher with %d classes" % (self.top, model.num_classes))
+        self.top, classes = int(top), _classes(model)
+        if not 1 <= self.top <= min(classes, HF._lib.TOP_MAX):
+            raise ValueError("top = %d of a teacher with %d classes" % (self.top, classes))
         self.codes = self.scale = None
         if int8_head:
             self.codes, self.scale = HF.quantize_rows(model.classifier.weight.detach())
@@ -201,8 +206,8 @@ def train(epoch, train_loader, model, criterion, optimizer, opt, lang_puller=Non
     if teacher is not None:
         if getattr(opt, "hip_graph", False):
             raise ValueError("opt.hip_graph captures the step without a teacher: run a distillation eagerly")
-        if teacher.model.num_classes > model.num_classes:
-            raise ValueError("the teacher knows %d classes, the student %d" % (teacher.model.num_classes, model.num_classes))
+        if _classes(teacher.model) > _classes(model):
+            raise ValueError("the teacher knows %d classes, the student %d" % (_classes(teacher.model), _classes(model)))
         if teacher.model is model:
             raise ValueError("a network cannot be its own teacher: load the frozen one as a second model")
     model.train()

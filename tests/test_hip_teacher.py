@@ -753,6 +753,8 @@ def test_pretraining_with_a_teacher(int8_head):
         pretrain.train(1, [], old, None, optimizer, opt, teacher=teacher)
     with pytest.raises(ValueError):
         pretrain.Teacher(old, top=21)
+    with pytest.raises(ValueError):
+        pretrain.Teacher(create_model("resnet12", -1, opt))
     small = create_model("resnet12", 10, opt).cuda()
     with pytest.raises(ValueError):
         pretrain.train(1, [], small, None, optimizer, opt, teacher=teacher)
