@@ -1304,6 +1304,11 @@ extern "C" int subreg_avgpool_bwd(const float* dfeat, void* dx, int B, int H, in
     return launch_status();
 }
 
+__global__ __launch_bounds__(BW_THREADS) void clear_f32_kernel(float* __restrict__ p, size_t n) {
+    const size_t i = (size_t)blockIdx.x * BW_THREADS + threadIdx.x;
+    if (i < n) p[i] = 0.f;
+}
+
 extern "C" int subreg_conv_wgrad_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype) {
     if (dtype != SUBREG_BF16 || ksize != 3 || B <= 0 || H <= 0 || W <= 0 || Cin <= 0 || Cout <= 0 || Cin % 32 || Cout % 32) return 1;
     const long long Q = (long long)B * (H + 2) * (W + 2);
@@ -1363,7 +1368,9 @@ extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed
         return launch_status();
     }
     // the kernels below accumulate into copy 0 with atomics; the caller adds all nsplit copies up
-    if (hipMemsetAsync(gw_packed, 0, sizeof(float) * (size_t)nsplit * Cout * taps * Cin, s) != hipSuccess) return SUBREG_EHIP;
+    // (cleared by a kernel: the step is captured into a graph, whose memset nodes have left old sums in place on later replays)
+    const size_t ngw = (size_t)nsplit * Cout * taps * Cin;
+    hipLaunchKernelGGL(clear_f32_kernel, bw_blocks(ngw), BW_THREADS, 0, s, gw_packed, ngw);
     if (dtype == SUBREG_BF16 && (taps == 1 || (pad_x && pad_dy))) {
         // bf16 MFMA path: 3x3 on zero-bordered copies (padded pixel coordinates), 1x1 directly on the compact tensors
         const __bf16 *xq = (const __bf16*)x, *dq = (const __bf16*)dy;

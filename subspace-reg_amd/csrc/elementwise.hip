@@ -618,13 +618,17 @@ extern "C" int subreg_mask_scale(const unsigned int* kept_count, long long numel
     return launch_status();
 }
 
+__global__ __launch_bounds__(EW_THREADS) void keep_all_kernel(unsigned char* __restrict__ keep, size_t n, unsigned int* __restrict__ kept_count) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *kept_count = 0;
+    for (size_t i = (size_t)blockIdx.x * EW_THREADS + threadIdx.x; i < n; i += (size_t)gridDim.x * EW_THREADS) keep[i] = 1;
+}
+
 extern "C" int subreg_dropblock_mask(const unsigned char* sample, unsigned char* keep_nhwc, int B, int C, int H, int W, int block_size,
                                      unsigned int* kept_count, void* stream) {
     SUBREG_CHECK_ARG(sample && keep_nhwc && kept_count && B > 0 && C > 0 && block_size >= 1 && H >= block_size && W >= block_size);
     hipStream_t s = (hipStream_t)stream;
     const size_t n = (size_t)B * C * H * W;
-    if (hipMemsetAsync(keep_nhwc, 1, n, s) != hipSuccess || hipMemsetAsync(kept_count, 0, sizeof(unsigned int), s) != hipSuccess)
-        return SUBREG_EHIP;
+    hipLaunchKernelGGL(keep_all_kernel, ew_blocks(n, 16), EW_THREADS, 0, s, keep_nhwc, n, kept_count);   // (no memset: a captured one is unsafe to replay)
     hipLaunchKernelGGL(dropblock_mask_kernel, 1, 1024, 0, s, sample, keep_nhwc, B, C, H, W, block_size);
     size_t blocks = (n + 256 * 64 - 1) / (256 * 64);
     if (blocks > 2048) blocks = 2048;
