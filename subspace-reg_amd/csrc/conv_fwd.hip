@@ -107,6 +107,15 @@ __device__ __forceinline__ void mma_step<float>(const uint4& a, const uint4& b, 
     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[3], fb[3], acc, 0, 0, 0);
 }
 
+// The statistics' squares are rounded before they are added: stated here, because whether the compiler fuses the two changes with the
+// instructions it may use, and the BatchNorm statistics (so every later step) with it.  Two whole-network SGD steps in f32 against the
+// reference's own: layer 1's first update is 8.4e-3 of itself away with rounded squares, 1.1e-2 with fused ones (near-ties of LeakyReLU
+// and MaxPool that fall the other way; neither form is the more exact one for the difference E[x^2] - E[x]^2 as a whole).
+__device__ __forceinline__ float rounded_square(float v) {
+#pragma clang fp contract(off)
+    return v * v;
+}
+
 // NI x NJ 32x32 accumulator blocks per wave (held as TR x TR MFMA tiles); WAVES_M x WAVES_N waves per workgroup; TPS taps staged per step
 // (one barrier per step); MINW = minimum waves per SIMD the register allocation must allow.
 // WK = 2: every output tile is owned by TWO waves that take alternate k-steps of each step and add their accumulators
@@ -766,7 +775,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N* WK * 64, MINW) void conv_fwd_kern
                         const float v = acc[i][j][r];
                         if (!raw_slab) y[(unsigned)(m * a.Cout + n)] = ElemTraits<T>::from_float(v);
                         s1 += v;
-                        s2 += v * v;
+                        s2 += rounded_square(v);
                     }
                 }
             }
