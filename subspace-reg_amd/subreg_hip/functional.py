@@ -235,6 +235,10 @@ def _rows(t, name):
         t = t.reshape(-1, t.shape[-1])
     if t.shape[0] >= 2 ** 22 or t.shape[1] > 2 ** 30:
         raise ValueError("%s: %d rows of %d; a call takes up to 2^22 - 1 rows of up to 2^30" % (name, t.shape[0], t.shape[1]))
+    return _row_major(t)
+
+
+def _row_major(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -351,14 +355,16 @@ _REDUCTION = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.RED
 
 
 def _distill_desc(z, tv, ti, target, temperature, kd_weight, ce_weight, ignore_index, reduction, ws):
-    d = _lib.DistillDesc()
-    d.logits, d.top_values, d.top_indices, d.target = z.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(target)
-    d.logits_stride, d.values_stride, d.indices_stride = z.stride(0), tv.stride(0), ti.stride(0)
-    d.dtype, d.values_dtype = _FLOAT_CODE[z.dtype], _FLOAT_CODE[tv.dtype]
-    d.rows, d.vocab, d.top = z.shape[0], z.shape[1], tv.shape[1]
-    d.temperature, d.kd_weight, d.ce_weight, d.ignore_index = temperature, kd_weight, ce_weight, ignore_index
-    d.reduction, d.ws, d.ws_bytes = reduction, ws.data_ptr(), ws.numel()
-    return d
+    return _lib.DistillDesc(z.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(target), z.stride(0), tv.stride(0), ti.stride(0),
+                            _FLOAT_CODE[z.dtype], _FLOAT_CODE[tv.dtype], z.shape[0], z.shape[1], tv.shape[1],
+                            temperature, kd_weight, ce_weight, ignore_index, reduction, 0, None, 0, None, None, ws.data_ptr(), ws.numel())
+
+
+def _kinds(z, tv, ti, target):
+    """What the kernel's bounds rest on."""
+    dev = z.device
+    return (z.shape, tv.shape, z.dtype, tv.dtype, dev, tv.device == dev and ti.device == dev and ti.shape == tv.shape,
+            ti.dtype, target is not None and (target.shape, target.dtype, target.device == dev))
 
 
 class DistillLossFn(torch.autograd.Function):
@@ -377,14 +383,23 @@ class DistillLossFn(torch.autograd.Function):
             dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
             d.dlogits = dz.data_ptr()
             ctx.save_for_backward(z, tv, ti, target)
-            ctx.dz, ctx.ws, ctx.desc = dz, ws, d         # (the saved tensors and ws keep what the descriptor points at)
+            ctx.dz, ctx.ws, ctx.desc = dz, ws, d
+            ctx.kinds = _kinds(z, tv, ti, target)
         _launch(dev, lib.subreg_distill_loss, "distill_loss", C.byref(d))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        z, d, dz = ctx.saved_tensors[0], ctx.desc, ctx.dz
+        d, dz = ctx.desc, ctx.dz
+        # Under saved-tensor hooks (checkpointing, offloading) these are other tensors than the forward's, which may be gone, and a
+        # hook may have laid them out anew.
+        saved = z, tv, ti, target = ctx.saved_tensors
+        if _kinds(*saved) != ctx.kinds:
+            raise RuntimeError("distill_loss: a saved tensor was unpacked with another shape, type or device")
+        z, tv, ti, target = _row_major(z), _row_major(tv), _row_major(ti), target if target is None else target.contiguous()
+        d.logits, d.top_values, d.top_indices, d.target = z.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(target)
+        d.logits_stride, d.values_stride, d.indices_stride = z.stride(0), tv.stride(0), ti.stride(0)
         g = g.reshape(-1)
         d.grad_scale, d.grad_scale_stride = g.data_ptr(), g.stride(0) if g.numel() > 1 else 0
         d.loss = None

@@ -615,6 +615,94 @@ def test_distill_gradient_against_differences():
     assert abs((ends[0] - ends[1]) / (2 * h) - slope) <= bound
 
 
+# ------------------------------------------------------------------------------------------------ saved-tensor hooks
+def test_distill_backward_reads_the_unpacked_tensors(monkeypatch):
+    """What the backward's call points at are the tensors that the unpack hook returned, not the forward's, which may be gone; a hook
+    that returns other shapes or types is refused (no kernel runs here: the calls are recorded)."""
+    calls = []
+
+    def record(dev, fn, what, ref):
+        d = ref._obj
+        calls.append((what, (d.logits, d.top_values, d.top_indices, d.target), (d.logits_stride, d.values_stride, d.indices_stride)))
+
+    monkeypatch.setattr(HF, "_launch", record)
+    for labels in (True, False):
+        z, tv = torch.randn(5, 9).requires_grad_(), torch.randn(5, 3)
+        ti, y = torch.randint(0, 9, (5, 3)), torch.randint(0, 9, (5,)) if labels else None
+        unpacked = []
+
+        def unpack(t):
+            # (rows further apart than the saved ones', and a last dimension that is not contiguous: both have to be followed)
+            n = torch.empty(t.shape[0], 2 * t[0].numel() + 1, dtype=t.dtype)[:, :2 * t[0].numel():2].view(t.shape) if t.dim() == 2 else t.clone()
+            unpacked.append(n.copy_(t))
+            return n
+
+        def far(t):
+            n = torch.empty(t.shape[0], t[0].numel() + 4, dtype=t.dtype)[:, :t[0].numel()] if t.dim() == 2 else t.clone()
+            unpacked.append(n.copy_(t))
+            return n
+
+        args = (2.0, 0.5, 0.5, -100, _lib.REDUCE_MEAN)
+        for hook in (lambda t: t, far, unpack):
+            calls.clear(), unpacked.clear()
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), hook):
+                loss = HF.DistillLossFn.apply(z, tv, ti, y, True, (), *args)
+            loss.backward()
+            assert [c[0] for c in calls] == ["distill_loss", "distill_loss(bwd)"]
+            assert all(a != b for a, b in zip(calls[0][1], calls[1][1]) if a)
+            assert (calls[1][1][3] is None) == (not labels)
+            if hook is far:
+                assert list(calls[1][1][:3 + labels]) == [t.data_ptr() for t in unpacked] and calls[1][2] == (13, 7, 7)
+            if hook is unpack:
+                assert calls[1][2] == (9, 3, 3)                      # rows with a contiguous last dimension were made of them
+        for wrong in (lambda t: t[:-1], lambda t: t.double() if t.dtype == torch.float32 else t.int()):
+            calls.clear()
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, wrong):
+                loss = HF.DistillLossFn.apply(z, tv, ti, y, True, (), *args)
+            with pytest.raises(RuntimeError, match="unpacked"):
+                loss.backward()
+            assert len(calls) == 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("factor", [1.0, 0.5, -3.0])
+@pytest.mark.parametrize("v", [60, 4100])
+def test_distill_under_saved_tensor_hooks(v, factor, dtype):
+    """Offloaded to the host, checkpointed and packed as copies: the gradient is that of the plain call, bit for bit, with the logits'
+    own memory given back and overwritten in between."""
+    from torch.utils.checkpoint import checkpoint
+    z, tv, ti, y = make_distill(9, v, 8, dtype, 4)
+
+    def loss_of(leaf, tv, ti, y):
+        return HF.distill_loss(leaf * 1, tv, ti, y, 2.0, 0.5, 0.5)       # (of a result, which only its saved form keeps)
+
+    leaf = z.detach().requires_grad_()
+    (factor * loss_of(leaf, tv, ti, y)).backward()
+    want = leaf.grad
+    _, plain = plain_distill(z, tv, ti, y, 2.0, 0.5, 0.5)
+    _, elem = distill_bounds(z, tv, ti, 2.0, 0.5, 0.5)
+    close(want, factor * plain, abs(factor) * elem, dtype, "gradient")
+
+    def clones():
+        return torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone())
+
+    for kind in ("cpu", "clone", "checkpoint"):
+        leaf = z.detach().requires_grad_()
+        mine = [t.clone() for t in (tv, ti, y)]
+        if kind == "checkpoint":
+            loss = checkpoint(loss_of, leaf, *mine, use_reentrant=False)
+        else:
+            with torch.autograd.graph.save_on_cpu() if kind == "cpu" else clones():
+                loss = loss_of(leaf, *mine)
+        if kind != "checkpoint":                                     # (a checkpoint keeps its function's arguments)
+            del mine
+        filler = [torch.full((9, v), 3, dtype=dtype, device="cuda") for _ in range(8)] + [torch.full((9, 8), 1, device="cuda") for _ in range(8)]
+        (factor * loss).backward()
+        assert torch.equal(leaf.grad, want), kind
+        del filler
+
+
 # ------------------------------------------------------------------------------------------------ far rows
 @gpu
 def test_rows_behind_the_32_bit_offsets():
