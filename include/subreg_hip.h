@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define SUBREG_ABI_VERSION 15
+#define SUBREG_ABI_VERSION 16
 
 #define SUBREG_OK 0
 #define SUBREG_EINVAL (-1)       /* bad argument (null pointer, shape not supported by contract) */
@@ -219,6 +219,13 @@ int subreg_pack_conv_weight_dgrad(const float* w_oihw, void* out, int Cout, int 
 int subreg_conv_wgrad_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype);
 int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W, int Cin,
                       int Cout, int ksize, int dtype, void* stream);
+/* The same without float atomics in bf16: 1x1 convolutions (and the first layer's K=32 form), whose K splits subreg_conv_wgrad adds into
+ * ONE copy in whatever order they end, store a copy each, so that a training step gives the same gradients bit for bit on every run.
+ * gw_packed: subreg_conv_wgrad_ordered_splits(...) copies, all written; unpack with that number.  What a 3x3 convolution does is the
+ * same in both forms.  f32 keeps its atomics (one copy). */
+int subreg_conv_wgrad_ordered_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype);
+int subreg_conv_wgrad_ordered(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W, int Cin,
+                              int Cout, int ksize, int dtype, void* stream);
 int subreg_unpack_wgrad(const float* gw_packed, float* grad_oihw, int Cout, int Cin, int ksize, int mode, int splits, void* stream);
 /* BatchNorm2d training-mode backward with the LeakyReLU' of `act` fused in (act == NULL: none):
  * g = dy*lrelu'(act); dgamma = sum g*xhat; dbeta = sum g; dx = gamma*invstd*(g - dbeta/N - xhat*dgamma/N).
@@ -273,7 +280,7 @@ typedef struct subreg_conv_train { /* per conv; every buffer caller-owned */
     float* bscale;        /* [cout] gamma*invstd of THIS batch */
     float* bshift;        /* [cout] beta - mean*gamma*invstd */
     const void* w_dgrad;  /* subreg_pack_conv_weight_dgrad output; NULL when no input gradient is needed */
-    float* gw_packed;     /* [splits][cout][taps][cin as the kernel sees it] fp32 scratch; the 3x3 convs may share one buffer, the 1x1
+    float* gw_packed;     /* [subreg_conv_wgrad_ordered_splits][cout][taps][cin as the kernel sees it] fp32 scratch; the 3x3 convs may share one buffer, the 1x1
                              shortcut convs another (with side_stream their branch can run while a 3x3 dW chain uses the first) */
     float* grad_w;        /* OIHW fp32: Conv2d.weight.grad */
     float* grad_gamma;    /* [cout] */

@@ -39,9 +39,9 @@ int bn_backward(const subreg_backbone_desc* d, const subreg_conv_desc& c, const 
 // the weight gradient of the conv that produced `raw`, from d(raw) and the conv's input
 int weight_grad(const subreg_backbone_desc* d, const subreg_train_desc* t, const subreg_conv_desc& c, const subreg_conv_train& tc,
                 const void* conv_input, const void* draw, int B, int H, int W, void* stream) {
-    TRY(subreg_conv_wgrad(conv_input, draw, tc.gw_packed, t->pad_x, t->pad_dy, B, H, W, c.cin, c.cout, c.ksize, d->dtype, stream));
+    TRY(subreg_conv_wgrad_ordered(conv_input, draw, tc.gw_packed, t->pad_x, t->pad_dy, B, H, W, c.cin, c.cout, c.ksize, d->dtype, stream));
     return subreg_unpack_wgrad(tc.gw_packed, tc.grad_w, c.cout, c.cin_raw, c.ksize_raw, c.cin_raw == 3 ? 1 : 0,
-                               subreg_conv_wgrad_splits(B, H, W, c.cin, c.cout, c.ksize, d->dtype), stream);
+                               subreg_conv_wgrad_ordered_splits(B, H, W, c.cin, c.cout, c.ksize, d->dtype), stream);
 }
 
 // Two-stream schedule of the step (subreg_train_desc.side_stream): the weight-gradient chain of a conv (pad copies, dW kernel,

@@ -420,11 +420,12 @@ __device__ __forceinline__ uint2 tr_read_off(unsigned addr) {
 
 // One workgroup = NCW waves: output channels [o0, o0+32) x input channels [c0, c0+32*NCW), all TAPS, over a range of padded
 // pixel rows.  Both operands are pixel-major in memory and in LDS; the MFMA wants 8 consecutive K (= pixels) per lane and
-// channel, which the transposing LDS read provides.  dW accumulated with fp32 atomics over the K splits.
+// channel, which the transposing LDS read provides.  Each K split stores a copy of its own, `part` elements apart (unpack adds them in a
+// fixed order: the same gradient bit for bit from run to run); part = 0: fp32 atomics on one copy, whose rounding depends on the order.
 template <int NCW, int TAPS>
 __global__ __launch_bounds__(NCW * 64, 2) void conv_wgrad_bf16_kernel(const __bf16* __restrict__ xq, const __bf16* __restrict__ dyq,
                                                                     float* __restrict__ gw, long long Q, int Wrow, int Cin,
-                                                                    int Cout, int rows_per_block) {
+                                                                    int Cout, int rows_per_block, long long part) {
     constexpr int KCH = 64;                              // pixel rows per chunk (4 MFMA k-steps)
     constexpr int NT = NCW * 64;
     constexpr int XS = NCW * 64 + 16, DS = 64 + 16;      // LDS row strides (bytes): 32 channels per wave / tile + 16 B pad
@@ -489,17 +490,41 @@ __global__ __launch_bounds__(NCW * 64, 2) void conv_wgrad_bf16_kernel(const __bf
         }
     }
     const int lr = lane & 31, lh = lane >> 5;
+    float* const out = gw + (size_t)blockIdx.y * (size_t)part;
 #pragma unroll
     for (int t = 0; t < TAPS; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int o = o0 + (r & 3) + 8 * (r >> 2) + 4 * lh;
-            atomicAdd(&gw[((size_t)o * TAPS + t) * Cin + c0 + wid * 32 + lr], acc[t][r]);
+            float* const at = out + ((size_t)o * TAPS + t) * Cin + c0 + wid * 32 + lr;
+            if (part) *at = acc[t][r];
+            else atomicAdd(at, acc[t][r]);
         }
 }
 
+// input channels of a workgroup of the kernel above, in 32s; 3x3: one (144 accumulator registers a wave: 8 waves per CU)
+static int wgrad_ncw(int Cin, int taps) { return taps == 9 ? 1 : Cin % 160 == 0 ? 5 : Cin % 64 == 0 ? 2 : 1; }
+
+// ~6 workgroups per CU in total.  dW + unpack in us at 64 images, a copy each | atomics on one copy: 84x84 32 -> 64 44 | 57, 42x42 64 -> 160
+// 31 | 45, 21x21 160 -> 320 32 | 50, 10x10 320 -> 640 29 | 46 (the atomics run at a quarter of the stores' rate; 768 workgroups with a copy
+// each 62, 39, 29, 25).
+constexpr int WGRAD_BLOCKS = 1536;
+
+// K splits of the kernel above with at most `most` workgroups' worth of them: rows of one split and their number.  A second call with
+// the number as `most` gives the same.
+static void wgrad_bf16_plan(long long Q, long long most, int* splits, int* rows_per_block) {
+    const long long rpb = ((Q + most - 1) / most + 63) / 64 * 64;
+    *rows_per_block = (int)rpb;
+    *splits = (int)((Q + rpb - 1) / rpb);
+}
+
+__global__ __launch_bounds__(BW_THREADS) void clear_f32_kernel(float* __restrict__ p, size_t n) {
+    const size_t i = (size_t)blockIdx.x * BW_THREADS + threadIdx.x;
+    if (i < n) p[i] = 0.f;
+}
+
 template <int NCW, int TAPS>
-static int launch_wgrad_bf16(const __bf16* xq, const __bf16* dyq, float* gw, long long Q, int Wrow, int Cin, int Cout,
+static int launch_wgrad_bf16(const __bf16* xq, const __bf16* dyq, float* gw, long long Q, int Wrow, int Cin, int Cout, int copies,
                              hipStream_t s) {
     const int halo = TAPS == 9 ? Wrow + 1 : 0;
     const size_t lds = (size_t)64 * (64 + 16) + (size_t)(64 + 2 * halo) * (NCW * 64 + 16);
@@ -508,11 +533,13 @@ static int launch_wgrad_bf16(const __bf16* xq, const __bf16* dyq, float* gw, lon
     static std::atomic<unsigned long long> lds_set{0};   // per instantiation
     if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), 160 * 1024, lds_set)) return rc;
     const int tiles = (Cout / 32) * (Cin / (32 * NCW));
-    long long splits = (1536 + tiles - 1) / tiles;                        // ~6 workgroups per CU in total
-    long long rpb = ((Q + splits - 1) / splits + 63) / 64 * 64;
-    if (rpb < 64) rpb = 64;
-    dim3 grid(tiles, (unsigned)((Q + rpb - 1) / rpb));
-    hipLaunchKernelGGL(kern, grid, dim3(NCW * 64), lds, s, xq, dyq, gw, Q, Wrow, Cin, Cout, (int)rpb);
+    const size_t n = (size_t)Cout * TAPS * Cin;
+    int splits, rpb;
+    wgrad_bf16_plan(Q, copies > 1 ? copies : (WGRAD_BLOCKS + tiles - 1) / tiles, &splits, &rpb);
+    if (copies > 1 && splits != copies) return SUBREG_EINVAL;                                  // (a copy nobody would write)
+    if (copies == 1 && splits > 1) hipLaunchKernelGGL(clear_f32_kernel, bw_blocks(n), BW_THREADS, 0, s, gw, n);
+    hipLaunchKernelGGL(kern, dim3(tiles, splits), dim3(NCW * 64), lds, s, xq, dyq, gw, Q, Wrow, Cin, Cout, rpb,
+                       copies > 1 || splits == 1 ? (long long)n : 0ll);
     return launch_status();
 }
 
@@ -1304,11 +1331,6 @@ extern "C" int subreg_avgpool_bwd(const float* dfeat, void* dx, int B, int H, in
     return launch_status();
 }
 
-__global__ __launch_bounds__(BW_THREADS) void clear_f32_kernel(float* __restrict__ p, size_t n) {
-    const size_t i = (size_t)blockIdx.x * BW_THREADS + threadIdx.x;
-    if (i < n) p[i] = 0.f;
-}
-
 extern "C" int subreg_conv_wgrad_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype) {
     if (dtype != SUBREG_BF16 || ksize != 3 || B <= 0 || H <= 0 || W <= 0 || Cin <= 0 || Cout <= 0 || Cin % 32 || Cout % 32) return 1;
     const long long Q = (long long)B * (H + 2) * (W + 2);
@@ -1318,19 +1340,28 @@ extern "C" int subreg_conv_wgrad_splits(int B, int H, int W, int Cin, int Cout, 
     return splits > 1 ? splits : 1;
 }
 
-extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W,
-                                 int Cin, int Cout, int ksize, int dtype, void* stream) {
+// copies of the deterministic form (see the header): the streaming 3x3 kernel's own; one a K split of the kernel for 1x1
+extern "C" int subreg_conv_wgrad_ordered_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype) {
+    const int stream = subreg_conv_wgrad_splits(B, H, W, Cin, Cout, ksize, dtype);
+    if (dtype != SUBREG_BF16 || ksize != 1 || B <= 0 || H <= 0 || W <= 0 || Cin <= 0 || Cout <= 0 || Cin % 32 || Cout % 32) return stream;
+    const int tiles = (Cout / 32) * (Cin / (32 * wgrad_ncw(Cin, 1)));
+    int splits, rpb;
+    wgrad_bf16_plan((long long)B * H * W, (WGRAD_BLOCKS + tiles - 1) / tiles, &splits, &rpb);
+    return splits;
+}
+
+static int conv_wgrad(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W,
+                      int Cin, int Cout, int ksize, int dtype, int nsplit, void* stream) {
     SUBREG_CHECK_ARG(x && dy && gw_packed && B > 0 && H > 0 && W > 0 && Cin > 0 && Cout > 0);
     SUBREG_CHECK_ARG((ksize == 1 || ksize == 3) && Cin % 32 == 0 && Cout % 32 == 0);
     hipStream_t s = (hipStream_t)stream;
     const int taps = ksize * ksize;
     const ConvGeom g = make_geom(B, H, W, taps, false);
-    const int nsplit = subreg_conv_wgrad_splits(B, H, W, Cin, Cout, ksize, dtype);
     // SUBREG_WGRAD_PADDED=1: the four-wave kernel on zero-bordered copies, as the one-wave kernel needs them (A/B runs)
     static const bool direct_on = [] { const char* e = getenv("SUBREG_WGRAD_PADDED"); return !(e && e[0] == '1'); }();
     const long long Qp = (long long)B * (H + 2) * (W + 2);
-    const bool direct = nsplit > 1 && wgrad_tile4() && direct_on && Qp < (1LL << 26);
-    if (nsplit > 1 && (direct || (pad_x && pad_dy))) {
+    const bool direct = taps == 9 && nsplit > 1 && wgrad_tile4() && direct_on && Qp < (1LL << 26);
+    if (taps == 9 && nsplit > 1 && (direct || (pad_x && pad_dy))) {
         // streaming bf16 3x3 kernel: per-split partial dW, no zero-fill, no atomics
         const long long Q = Qp;
         int splits, rpb;
@@ -1367,10 +1398,6 @@ extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed
                            Q, W + 2, Cin, Cout, rpb, ring);
         return launch_status();
     }
-    // the kernels below accumulate into copy 0 with atomics; the caller adds all nsplit copies up
-    // (cleared by a kernel: the step is captured into a graph, whose memset nodes have left old sums in place on later replays)
-    const size_t ngw = (size_t)nsplit * Cout * taps * Cin;
-    hipLaunchKernelGGL(clear_f32_kernel, bw_blocks(ngw), BW_THREADS, 0, s, gw_packed, ngw);
     if (dtype == SUBREG_BF16 && (taps == 1 || (pad_x && pad_dy))) {
         // bf16 MFMA path: 3x3 on zero-bordered copies (padded pixel coordinates), 1x1 directly on the compact tensors
         const __bf16 *xq = (const __bf16*)x, *dq = (const __bf16*)dy;
@@ -1381,16 +1408,20 @@ extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed
             hipLaunchKernelGGL(pad_copy_kernel, bw_blocks((size_t)Q * Cout / 8), BW_THREADS, 0, s, (const __bf16*)dy, (__bf16*)pad_dy, B, H, W, Cout);
             xq = (const __bf16*)pad_x; dq = (const __bf16*)pad_dy;
         }
-#define WGB(NCW) (taps == 9 ? launch_wgrad_bf16<NCW, 9>(xq, dq, gw_packed, Q, W + 2, Cin, Cout, s) \
-                            : launch_wgrad_bf16<NCW, 1>(xq, dq, gw_packed, Q, W + 2, Cin, Cout, s))
+#define WGB(NCW) launch_wgrad_bf16<NCW, 1>(xq, dq, gw_packed, Q, W + 2, Cin, Cout, nsplit, s)
         int rc;
-        if (taps == 9) rc = WGB(1);           // 144 accumulator registers per wave: one-wave workgroups keep 8 waves per CU
-        else if (Cin % 160 == 0) rc = WGB(5);
-        else if (Cin % 64 == 0) rc = WGB(2);
-        else rc = WGB(1);
+        switch (wgrad_ncw(Cin, taps)) {
+            case 5: rc = WGB(5); break;
+            case 2: rc = WGB(2); break;
+            default: rc = taps == 9 ? launch_wgrad_bf16<1, 9>(xq, dq, gw_packed, Q, W + 2, Cin, Cout, nsplit, s) : WGB(1); break;
+        }
 #undef WGB
         if (rc != SUBREG_EUNSUPPORTED) return rc;
     }
+    // the kernel below accumulates into copy 0 with atomics; the caller adds all nsplit copies up
+    // (cleared by a kernel: the step is captured into a graph, see tests/test_hip_replay.py)
+    const size_t ngw = (size_t)nsplit * Cout * taps * Cin;
+    hipLaunchKernelGGL(clear_f32_kernel, bw_blocks(ngw), BW_THREADS, 0, s, gw_packed, ngw);
     const int tiles = (Cout / 32) * (Cin / 32);
     // enough waves to fill the chip, but at least 64 pixels per wave
     long long ppw = ((long long)g.npix * tiles + 8191) / 8192;
@@ -1404,6 +1435,18 @@ extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed
     else return SUBREG_EINVAL;
 #undef WG
     return launch_status();
+}
+
+extern "C" int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W,
+                                 int Cin, int Cout, int ksize, int dtype, void* stream) {
+    return conv_wgrad(x, dy, gw_packed, pad_x, pad_dy, B, H, W, Cin, Cout, ksize, dtype,
+                      subreg_conv_wgrad_splits(B, H, W, Cin, Cout, ksize, dtype), stream);
+}
+
+extern "C" int subreg_conv_wgrad_ordered(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W,
+                                         int Cin, int Cout, int ksize, int dtype, void* stream) {
+    return conv_wgrad(x, dy, gw_packed, pad_x, pad_dy, B, H, W, Cin, Cout, ksize, dtype,
+                      subreg_conv_wgrad_ordered_splits(B, H, W, Cin, Cout, ksize, dtype), stream);
 }
 
 extern "C" int subreg_unpack_wgrad(const float* gw_packed, float* grad_oihw, int Cout, int Cin, int ksize, int mode, int splits,

@@ -19,7 +19,7 @@ CONV_KERNEL_GENERAL, CONV_KERNEL_WIDE = 256, 512   # kernel selection of subreg_
 CONV_KERNEL_WIDE_ALT = 1024                        # with _WIDE: the other MFMA shape of conv_wide.hip than its default for the problem
 CONV_KERNEL_WIDE_128, CONV_KERNEL_WIDE_256 = 2048, 4096   # with _WIDE: the 128- / 256-row tiling of conv_wide16_kernel
 FWD_TRAIN = 1
-ABI_VERSION = 15
+ABI_VERSION = 16
 I8_MAX_DIM, TOP_MAX = 131071, 256            # SUBREG_I8_MAX_DIM, SUBREG_TOP_MAX
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
 DISTILL_SKIP_UNIT, DISTILL_COUNTED = 1, 2
@@ -122,6 +122,8 @@ SIGNATURES = {
     "subreg_pack_conv_weight_dgrad": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "subreg_conv_wgrad": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "subreg_conv_wgrad_splits": (_I, [_I, _I, _I, _I, _I, _I, _I]),
+    "subreg_conv_wgrad_ordered": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "subreg_conv_wgrad_ordered_splits": (_I, [_I, _I, _I, _I, _I, _I, _I]),
     "subreg_validate_sets": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _P]),
     "subreg_softmax_ce": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P]),
     "subreg_semantic_target": (_I, [_P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _P, _P]),

@@ -59,7 +59,7 @@ class TrainStash:
                     setattr(tc, f, self.named[(bi, slot, f)].data_ptr())
                 kin = 32 if ci == 3 else ci
                 kk = 1 if ci == 3 else k
-                nsplit = lib.subreg_conv_wgrad_splits(B, h, w, kin, cout, kk, hb.dtype)
+                nsplit = lib.subreg_conv_wgrad_ordered_splits(B, h, w, kin, cout, kk, hb.dtype)
                 if slot == "down":
                     gw_down_need = max(gw_down_need, nsplit * cout * kk * kk * kin)
                 else:

@@ -62,3 +62,60 @@ def test_replayed_conv_wgrad_starts_from_zero(ksize, dtype):
         run()                                                              # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(gw, want), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 84, 84, 32, 64), (64, 21, 21, 160, 320), (5, 10, 10, 320, 640), (3, 7, 9, 64, 96), (1, 1, 1, 32, 32),
+                                   (2, 5, 13, 96, 32), (11, 42, 42, 64, 160)])
+def test_ordered_conv_wgrad_repeats_bit_for_bit(shape):
+    """1x1 dW with a copy for each K split: every copy is written, the sum is the definition's, and every run gives the same bits."""
+    from subreg_hip import _lib
+    lib = _lib.load()
+    B, H, W, Cin, Cout = shape
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(B * H * W, Cin, generator=g, device="cuda").bfloat16()
+    dy = torch.randn(B * H * W, Cout, generator=g, device="cuda").bfloat16()
+    n = lib.subreg_conv_wgrad_ordered_splits(B, H, W, Cin, Cout, 1, _lib.BF16)
+    gw = torch.empty(n * Cout * Cin, dtype=torch.float32, device="cuda")
+    grad = torch.empty(Cout, Cin, device="cuda")
+    first = None
+    for _ in range(5):
+        gw.fill_(float("nan"))
+        _lib.check(lib.subreg_conv_wgrad_ordered(_lib.ptr(x), _lib.ptr(dy), _lib.ptr(gw), None, None, B, H, W, Cin, Cout, 1, _lib.BF16,
+                                                 _lib.stream_ptr()))
+        _lib.check(lib.subreg_unpack_wgrad(_lib.ptr(gw), _lib.ptr(grad), Cout, Cin, 1, 0, n, _lib.stream_ptr()))
+        first = grad.clone() if first is None else first
+        assert torch.equal(grad, first)
+    want = dy.double().t() @ x.double()
+    # products of bf16 numbers are exact in fp32; an element's chain: the rows of a split, then the copies
+    bound = 2.0 ** -24 * (B * H * W / n + 64 + n) * (dy.double().abs().t() @ x.double().abs())
+    assert bool(((grad.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_training_steps_repeat_bit_for_bit():
+    """Two whole pretraining steps in bf16, twice from the same start: the same parameters.  (With sums that depend on the order of
+    float atomics the second step's bf16 weights now and then round the other way, and parameters part by 1e-2.)"""
+    from types import SimpleNamespace
+
+    from subreg_hip import synthetic as syn
+    from subreg_hip.resnet_language import create_model
+    from subreg_hip.train import SGD
+
+    def run():
+        net = create_model("resnet18", 60, SimpleNamespace(no_dropblock=True, linear_bias=False, hip_dtype="bf16"))
+        net.load_state_dict({k: torch.from_numpy(np.array(v)) for k, v in syn.make_state_dict(1, randomize_bn=False).items()})
+        net = net.cuda().train()
+        opt = SGD(net.parameters(), lr=0.05, momentum=0.9, weight_decay=5e-4)
+        from oracle.resnet_ref import MaskSource
+        for s in range(2):
+            x = torch.from_numpy(syn.make_images(10 + s, 9, 32)).cuda()
+            y = torch.from_numpy(np.random.RandomState(20 + s).randint(0, 60, 9)).cuda()
+            net.mask_source = MaskSource(s)
+            opt.zero_grad()
+            torch.nn.functional.cross_entropy(net(x), y).backward()
+            opt.step()
+        return {k: v.detach().clone() for k, v in net.named_parameters()}
+
+    a, b = run(), run()
+    assert [k for k in a if not torch.equal(a[k], b[k])] == []

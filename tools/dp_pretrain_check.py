@@ -2,8 +2,8 @@
 """Data-parallel pretraining check on ONE GPU: two processes (gloo; on an 8-GPU node the same code runs with backend nccl =
 RCCL over xGMI, one GPU per rank) each take their share of a global batch, back-propagate loss * n_local / n_global through
 the STAGED backward (GradientSync.stage_ready all-reduces each stage's gradient range while the earlier blocks' backward is
-still queued), finish with the classifier, and step the fused SGD.  The result must equal - up to the run-to-run noise of the float atomics in
-the 1x1 convolutions' weight gradients, which the tool measures - a single process that does what nn.DataParallel does (train_supervised.py:141-142): the same two shards through the same replica code (BatchNorm
+still queued), finish with the classifier, and step the fused SGD.  The result must equal (the step is deterministic in bf16; the tool
+measures what two runs of the same process differ by) a single process that does what nn.DataParallel does (train_supervised.py:141-142): the same two shards through the same replica code (BatchNorm
 statistics per replica), gradients summed, one optimiser step.  Uneven shards (7 = 4 + 3) are part of the check.
 
   python tools/dp_pretrain_check.py        (the parent never touches the GPU; it only starts the workers)
@@ -70,9 +70,9 @@ def worker(rank, world, port, q):
     dp = {k: v.detach().cpu() for k, v in net.named_parameters()}
     calls = sync.calls
     dist.barrier()
-    # ---- rank 0 alone: both shards through one replica, gradients summed (what DataParallel computes).  Twice: the 1x1
-    #      shortcut convolutions' weight gradients are accumulated with float atomics (order-dependent rounding), so two
-    #      runs of the SAME single-process code differ in the last bit - the yardstick for the two-rank result
+    # ---- rank 0 alone: both shards through one replica, gradients summed (what DataParallel computes).  Twice: what two
+    #      runs of the SAME single-process code differ by (nothing, where no kernel's sums depend on an order) is the
+    #      yardstick for the two-rank result
     if rank == 0:
         def emulate():
             ref = make()
@@ -121,7 +121,7 @@ def main():
     ok = d_dp <= max(4 * d_self, 1e-6 * scale)
     print("data-parallel pretraining, 2 ranks x 1 GPU (gloo), global batch %d = 4 + 3, %d steps, staged + overlapped all-reduce "
           "(%d collectives): max |parameter difference| to the single-process DataParallel emulation %.3g; two runs of that "
-          "emulation differ by %.3g (float atomics in the 1x1 weight gradients); parameter scale %.3g -> %s" %
+          "emulation differ by %.3g; parameter scale %.3g -> %s" %
           (N_GLOBAL, STEPS, calls, d_dp, d_self, scale, "EQUIVALENT" if ok else "MISMATCH"))
     sys.exit(0 if ok else 1)
 
