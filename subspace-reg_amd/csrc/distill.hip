@@ -385,6 +385,7 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
             s_cnt[1] = (float)max(n_ce, 1);
         }
     }
+    if constexpr (NT == 64) __syncthreads();         // (a block of one wave passes no barrier in its reductions, which order s_cnt elsewhere)
 
     // the student's softmax
     auto add = [](float p, float q) { return p + q; };
