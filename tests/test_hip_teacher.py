@@ -304,6 +304,28 @@ def test_linear_int8_largest_sums_are_exact():
         assert torch.equal(got.cpu(), want.expand(2, 3))
 
 
+# The loops of every kernel at work: tiles of each size with three and more stages of K (whole and ragged edges, out a multiple of 4 or
+# not), one row with more channels than the grid has waves for (each length of the row in registers), few rows with more groups of
+# channels than the grid has blocks (each number of row tiles), and short rows of many channels, which go to the tiles.
+STEADY = [(4096, 512, 3584), (4000, 521, 3601), (3990, 1153, 3600), (2304, 640, 2048), (2250, 777, 2101), (1024, 640, 2048),
+          (1000, 650, 2049), (300, 1000, 521), (1, 1000, 40000), (1, 2047, 33001), (1, 4096, 20000), (1, 8192, 9001),
+          (5, 2100, 70001), (20, 2048, 66000), (40, 2176, 66001), (64, 2100, 65999), (64, 1024, 32768), (9, 1500, 20003)]
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", STEADY)
+def test_linear_int8_steady_state_is_exact(m, k, n):
+    """Codes given and scales of 1: every product is the integer sum, rounded to fp32 once (64-bit floats hold the sums exactly)."""
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
+    pitch = (k + 15) // 16 * 16                                      # rows as quantize_rows lays them out: read by the tiles as they are
+    w = torch.randint(-128, 128, (n, pitch), generator=g, dtype=torch.int8, device="cuda")[:, :k]
+    got = HF.linear_int8(x, w, torch.ones(n, device="cuda"), None, torch.ones(m, device="cuda"))
+    for lo in range(0, n, 8192):
+        want = x.double() @ w[lo:lo + 8192].double().t().contiguous()
+        assert torch.equal(got[:, lo:lo + 8192], want.float()), lo
+
+
 @gpu
 def test_linear_int8_strides_and_leading_dimensions():
     x, wf = rnd((4, 6, 200), 1), rnd((90, 200), 2)
