@@ -493,7 +493,9 @@ int subreg_top_logits(const void* logits, long long stride, int dtype, int rows,
  * ignore_index, makes the row's loss and gradient NaN; nothing is read or written out of range.
  * loss (optional) and dlogits (optional, [rows][vocab] contiguous, dtype of the logits): the gradient times grad_scale[i * grad_scale_stride]
  * (NULL: 1).  flags: SUBREG_DISTILL_SKIP_UNIT - rows whose grad_scale is exactly 1 are left as they are (they hold this gradient
- * already); SUBREG_DISTILL_COUNTED - `ws` is the one a call with the same rows, top and reduction has filled. */
+ * already); SUBREG_DISTILL_COUNTED - `ws` is as a call with dlogits left it that differs from this one at most in grad_scale, its stride,
+ * loss, dlogits and flags (SUBREG_MEAN keeps its two row counts there; which calls make them, and where, depends on everything else:
+ * a call for the loss alone makes none).  Without the flag every call counts for itself. */
 #define SUBREG_NONE 0
 #define SUBREG_SUM 1
 #define SUBREG_MEAN 2

@@ -623,6 +623,39 @@ def test_distill_second_backward_and_changed_inputs():
 
 
 @gpu
+@pytest.mark.parametrize("v", [60, 3000, 140003])
+@pytest.mark.parametrize("reduction", [_lib.REDUCE_SUM, _lib.REDUCE_MEAN])
+def test_distill_counted_workspace(v, reduction):
+    """The C entry with counts that an earlier gradient call left: the same bits as a call that counts for itself, with the logits' rows
+    elsewhere and another factor."""
+    lib, n, k = _lib.load(), 300, 9
+    z, tv, ti, y = make_distill(n, v, k, torch.float32, 12)
+    ti[5], y[7] = -1, -100
+    moved = torch.zeros(n, v + 5, device="cuda")
+    moved[:, :v] = z
+    ws = [torch.empty(lib.subreg_distill_ws_bytes(n), dtype=torch.uint8, device="cuda").fill_(0x5a) for _ in range(2)]
+    loss, factor = torch.empty(1, device="cuda"), torch.full((1,), 0.375, device="cuda")
+
+    def call(rows, ws, flags, **out):
+        d = _lib.DistillDesc(logits=rows.data_ptr(), top_values=tv.data_ptr(), top_indices=ti.data_ptr(), target=y.data_ptr(),
+                             logits_stride=rows.stride(0), values_stride=k, indices_stride=k, dtype=0, values_dtype=0, rows=n, vocab=v,
+                             top=k, temperature=2.0, kd_weight=0.5, ce_weight=0.5, ignore_index=-100, reduction=reduction, flags=flags,
+                             ws=ws.data_ptr(), ws_bytes=ws.numel(), **{name: t.data_ptr() for name, t in out.items()})
+        _lib.check(lib.subreg_distill_loss(ctypes.byref(d), _lib.stream_ptr()), "distill_loss")
+
+    a, b, c = (torch.empty(n, v, device="cuda") for _ in range(3))
+    call(z, ws[0], 0, loss=loss, dlogits=a)
+    call(moved[:, :v], ws[0], _lib.DISTILL_COUNTED, dlogits=b, grad_scale=factor)
+    call(z, ws[1], 0, dlogits=c, grad_scale=factor)
+    assert torch.equal(b, c)
+    want, grad = plain_distill(z, tv, ti, y, 2.0, 0.5, 0.5, reduction="sum" if reduction == _lib.REDUCE_SUM else "mean")
+    row, elem = distill_bounds(z, tv, ti, 2.0, 0.5, 0.5)
+    close(loss, want.reshape(1), row * (n if reduction == _lib.REDUCE_SUM else 2), note="loss")
+    close(a, grad, elem, note="gradient")
+    close(b, 0.375 * grad, 0.375 * elem, note="gradient with a factor")
+
+
+@gpu
 def test_distill_gradient_against_differences():
     z, tv, ti, y = make_distill(6, 77, 5, torch.float32, 8, scale=1.0)
     leaf = z.detach().requires_grad_()
