@@ -509,7 +509,7 @@ typedef struct {
     long long logits_stride, values_stride, indices_stride;
     int dtype, values_dtype;
     int rows, vocab, top;          /* top <= SUBREG_TOP_MAX */
-    float temperature, kd_weight, ce_weight;
+    float temperature, kd_weight, ce_weight;   /* 1e-30 <= temperature <= 1e15, |kd_weight| * max(temperature, temperature^2) <= 1e30, |ce_weight| <= 1e30 */
     long long ignore_index;
     int reduction, flags;
     const float* grad_scale;

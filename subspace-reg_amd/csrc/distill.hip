@@ -1,6 +1,8 @@
 // Distillation from a teacher's top logits with the labels' cross entropy, loss and gradient in one pass over the student's logits.
 //   p = softmax over a row's kept entries of t / T;  e_v = exp((z_v - m) / T), S = sum_v e_v;  likewise at T = 1 for the labels
 //   KL = sum_j p_j (log p_j - (z_{i_j} - m) / T + log S);        CE = log S_1 - (z_y - m)
+//   T KL = sum_j p_j ((t_j - t_m) - (z_{i_j} - m)) + T (log S - log P): what a row's term is kept as (T^2 alone overflows before the loss
+//   does, and a difference over T where a kept entry's logit is masked by the type's lowest number)
 //   d(a T^2 KL)/dz_v = a T (e_v / S - sum_{j: i_j = v} p_j);     d(b CE)/dz_v = b (e1_v / S_1 - [v = y])
 // Every row needs its maximum and two sums before its first gradient is known, so a row is read, reduced and written by one block, and
 // held in its registers in between: each logit is read once and each gradient written once.  Bound by memory: 4096 x 32000 bf16 with
@@ -34,7 +36,7 @@ struct DistillArgs {
     long long gs_stride;
     float* loss;
     void* dz;
-    float* row_kd;                       // [rows] KL of the row (SUM / MEAN)
+    float* row_kd;                       // [rows] T KL of the row (SUM / MEAN)
     float* row_ce;
     int* counts;                         // [count_blocks][2] rows with entries | with a label (MEAN)
 };
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(DistillArgs a) {
         if (lane == 0) {
             const bool mean = a.reduction == SUBREG_MEAN;
             const double kd = mean ? v[0] / fmax(v[2], 1.0) : v[0], ce = mean ? v[1] / fmax(v[3], 1.0) : v[1];
-            a.loss[0] = (float)((double)a.kd * a.temp * a.temp * kd + (double)a.ce * ce);
+            a.loss[0] = (float)((double)a.kd * a.temp * kd + (double)a.ce * ce);
         }
     }
 }
@@ -230,13 +232,13 @@ __device__ __forceinline__ void distill_any_row(const DistillArgs& a, long long 
             const float p = s_p[j];
             if (s_i[j] < 0 || p == 0.f) continue;
             const float tv = ElemTraits<TV>::to_float(((const TV*)a.tv)[r * a.tv_stride + j]);
-            term += p * (((tv - tm) - (ElemTraits<T>::to_float(z[s_i[j]]) - m)) * a.inv_t + (logf(se) - logf(ps)));
+            term += p * (((tv - tm) - (ElemTraits<T>::to_float(z[s_i[j]]) - m)) + a.temp * (logf(se) - logf(ps)));
         }
         term = block_reduce(term, red, 0.f, add);
         if (tid == 0) {
             if (bad) term = NAN;
             const float ce = !ce_on ? 0.f : bad_y ? NAN : logf(s1) - (ElemTraits<T>::to_float(z[y]) - m);
-            if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
+            if (out) out[r] = a.kd * a.temp * term + a.ce * ce;
             else { a.row_kd[r] = kd_on ? term : NO_TERM; a.row_ce[r] = ce_on ? ce : NO_TERM; }
         }
     }
@@ -471,22 +473,23 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
 
     constexpr float LN2 = 0.69314718055994530942f;
     if (a.loss && wid == 0) {
-        const float ls = log2f(se), lp = log2f(ps);
+        const float off = fmaf(m, a.c_t, -mc);       // what rounding m c left out: common to the exponents, but not to z - m
+        const float t_ls = a.temp * LN2 * (log2f(se) - off - log2f(ps));
         float term = 0.f;
 #pragma unroll
         for (int q = 0; q < EPL; ++q)
             if (p[q] > 0.f || p[q] != p[q])
-                term += p[q] * (((tv[q] - tm) * a.c_t - lp) - (fmaf(z_at[q], a.c_t, -mc) - ls)) * LN2;
+                term += p[q] * (((tv[q] - tm) - (z_at[q] - m)) + t_ls);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) term += __shfl_xor(term, o);
         if (lane == 0) {
             if (bad) term = NAN;
             float ce = 0.f;
             if (ce_on) {
-                const float xy = SQ < 0 ? fmaf(z_y, LOG2E, -mc1) : fmaf(z_y, a.c_t, -mc) * (float)(1 << max(SQ, 0));
-                ce = bad_y ? NAN : (log2f(s1) - xy) * LN2;
+                const float off1 = SQ < 0 ? fmaf(m, LOG2E, -mc1) : off * (float)(1 << max(SQ, 0));
+                ce = bad_y ? NAN : (log2f(s1) - off1) * LN2 - (z_y - m);
             }
-            if (out) out[r] = a.kd * a.temp * a.temp * term + a.ce * ce;
+            if (out) out[r] = a.kd * a.temp * term + a.ce * ce;
             else { a.row_kd[r] = kd_on ? term : NO_TERM; a.row_ce[r] = ce_on ? ce : NO_TERM; }
         }
     }
@@ -608,7 +611,8 @@ extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     SUBREG_CHECK_ARG(d && d->logits && d->top_values && d->top_indices && (d->loss || d->dlogits));
     SUBREG_CHECK_ARG(d->rows > 0 && d->rows <= MAX_ROWS && d->vocab > 0 && d->vocab <= MAX_COLUMNS && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
     SUBREG_CHECK_ARG(d->logits_stride >= 0 && d->values_stride >= 0 && d->indices_stride >= 0 && d->grad_scale_stride >= 0);
-    SUBREG_CHECK_ARG(float_dtype(d->dtype) && float_dtype(d->values_dtype) && d->temperature > 0.f && d->temperature <= 3.0e38f);
+    SUBREG_CHECK_ARG(float_dtype(d->dtype) && float_dtype(d->values_dtype) && d->temperature >= 1e-30f && d->temperature <= 1e15f);
+    SUBREG_CHECK_ARG(fabs((double)d->kd_weight) * d->temperature * fmax(d->temperature, 1.0) <= 1e30 && fabs((double)d->ce_weight) <= 1e30);
     SUBREG_CHECK_ARG(d->reduction >= SUBREG_NONE && d->reduction <= SUBREG_MEAN);
     SUBREG_CHECK_ARG(!(d->flags & SUBREG_DISTILL_SKIP_UNIT) || (d->grad_scale && d->dlogits && !d->loss));
     SUBREG_CHECK_ARG(d->ws && ((size_t)d->ws & 255) == 0 && d->ws_bytes >= subreg_distill_ws_bytes(d->rows));

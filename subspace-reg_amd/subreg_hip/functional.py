@@ -423,7 +423,7 @@ def distill_loss(logits, top_values, top_indices, target=None, temperature=1.0, 
     ignore_index no second; a row with neither is not read, its gradient is 0.  reduction "mean": each term over the rows that have it
     (no such row: 0); "sum"; "none": [...].  Gradient for the logits only, in their type;
     inside a captured graph take it with torch.autograd.grad (as train.GraphedStep does), not with backward().  An index >= V, or a target outside
-    [0, V), makes its row's loss and gradient NaN."""
+    [0, V), makes its row's loss and gradient NaN.  temperature: 1e-30 ... 1e15, with kd_weight * temperature ** 2 up to 1e30."""
     _float_code(logits, "logits")
     _float_code(top_values, "top_values")
     lead = logits.shape[:-1]
@@ -437,10 +437,10 @@ def distill_loss(logits, top_values, top_indices, target=None, temperature=1.0, 
     if reduction not in _REDUCTION:
         raise ValueError("reduction must be 'none', 'sum' or 'mean', got %r" % (reduction,))
     temperature, kd_weight, ce_weight = float(temperature), float(kd_weight), float(ce_weight)
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError("temperature must be a positive number, got %r" % temperature)
-    if not abs(kd_weight) <= 1e30 or not abs(ce_weight) <= 1e30:
-        raise ValueError("kd_weight and ce_weight must be finite")
+    if not 1e-30 <= temperature <= 1e15:
+        raise ValueError("temperature must lie in 1e-30 ... 1e15, got %r" % temperature)
+    if not abs(kd_weight) * temperature * max(temperature, 1.0) <= 1e30 or not abs(ce_weight) <= 1e30:
+        raise ValueError("kd_weight * temperature ** 2 and ce_weight must be numbers up to 1e30")
     z, tv, ti = _rows(logits, "logits"), _rows(top_values.detach(), "top_values"), _rows(top_indices, "top_indices").to(torch.int64)
     if tv.shape[1] > _lib.TOP_MAX:
         raise ValueError("%d entries a row: at most %d are served" % (tv.shape[1], _lib.TOP_MAX))

@@ -622,6 +622,62 @@ def test_distill_second_backward_and_changed_inputs():
     assert not HF.distill_loss(z, tv, ti, y).requires_grad
 
 
+def test_distill_temperature_range_on_cpu():
+    f = torch.zeros
+    good = dict(logits=f(2, 8), top_values=f(2, 3), top_indices=f(2, 3, dtype=torch.int64))
+    for bad in (dict(temperature=1e16), dict(temperature=1e-31), dict(temperature=1e12, kd_weight=1e7), dict(kd_weight=1e31)):
+        with pytest.raises(ValueError):
+            HF.distill_loss(**good, **bad)
+    for edge in (dict(temperature=1e15), dict(temperature=1e-30), dict(temperature=1e12, kd_weight=1e5), dict(temperature=0.5, kd_weight=1e30)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            HF.distill_loss(**good, **edge)
+    lib, p = _lib.load(), 1 << 20
+    for t, kd, ce in ((1e16, 1.0, 0.0), (1e-31, 1.0, 0.0), (math.inf, 1.0, 0.0), (1e12, 1e7, 0.0), (1.0, math.nan, 0.0), (1.0, 1.0, 1e31)):
+        d = _lib.DistillDesc(logits=p, top_values=p, top_indices=p, logits_stride=8, values_stride=3, indices_stride=3, rows=2, vocab=8,
+                             top=3, temperature=t, kd_weight=kd, ce_weight=ce, reduction=2, loss=p, ws=p, ws_bytes=lib.subreg_distill_ws_bytes(2))
+        assert lib.subreg_distill_loss(ctypes.byref(d), None) == -1, (t, kd, ce)
+
+
+@gpu
+@pytest.mark.parametrize("v", [5, 60, 3001, 140003])
+@pytest.mark.parametrize("temp", [1e-30, 1e-12, 1e-3, 1e3, 1e10, 1e15])
+def test_distill_temperature_range(v, temp):
+    """The ends of the accepted range: nothing overflows that the loss itself does not."""
+    z, tv, ti, y = make_distill(6, v, 4, torch.float32, 3)
+    for reduction in ("none", "sum", "mean"):
+        check_distill(z, tv, ti, y, temp, 1.0, 0.5, reduction)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("v", [7, 300, 4100, 50021, 140003])
+@pytest.mark.parametrize("temp", [0.25, 1.0, 2.0, 3.0])
+def test_distill_kept_entries_and_labels_at_the_lowest_number(v, temp, dtype):
+    """A student masked by its type's lowest number where the teacher has a share, or the label is: the loss is that large, not
+    infinite."""
+    z, _, _, _ = make_distill(3, v, 4, dtype, 6)
+    low = torch.finfo(dtype).min
+    z[:, 4:] = low
+    ti = torch.tensor([[0, 1, 2, 5], [3, 5, 6, 0], [0, 1, 2, 3]]).cuda()
+    tv = torch.tensor([[1.0, 0.5, 0.0, -1.0], [2.0, -2.0, -3.0, 1.0], [0.0, 0.0, 0.0, 0.0]]).cuda().to(dtype)
+    y = torch.tensor([1, 0, 6]).cuda()
+    # (T p < 0.7 for the masked entries, ce = 1/4: every row's loss fits fp32.)  At such numbers a bound is relative: differences,
+    # products and sums of at most four shares, each rounded, and the shares' own error, where exponents reach 5 / T
+    many = U * (64 + 4 * 5 / temp)
+    for kd, ce in ((1.0, 0.0), (0.25, 0.25)):
+        leaf = z.detach().requires_grad_()
+        loss = HF.distill_loss(leaf, tv, ti, y, temp, kd, ce, reduction="none")
+        loss.sum().backward()
+        want, grad = plain_distill(z, tv, ti, y, temp, kd, ce, reduction="none")
+        assert float(want.max()) > 1 and bool(torch.isfinite(want.float()).all())
+        near = torch.where(z == low, z[:, :4].float().min().to(dtype), z)
+        row, elem = distill_bounds(near, tv, ti, temp, kd, ce)
+        close(loss, want, row + many * want, note="loss")
+        close(leaf.grad, grad, elem, dtype, "gradient")
+        with torch.no_grad():
+            close(HF.distill_loss(leaf, tv, ti, y, temp, kd, ce, reduction="none"), want, row + many * want, note="the loss alone")
+
+
 @gpu
 @pytest.mark.parametrize("v", [60, 3000, 140003])
 @pytest.mark.parametrize("reduction", [_lib.REDUCE_SUM, _lib.REDUCE_MEAN])
