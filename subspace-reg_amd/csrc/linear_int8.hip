@@ -87,26 +87,30 @@ __global__ __launch_bounds__(256) void quantize_any_rows_kernel(const T* __restr
 }
 
 // codes copied to rows of the padded pitch (x given as codes, weights whose rows start anywhere): a thread per 16 bytes, which are read
-// at any address; the bytes of a row's last ones behind `dim`, and those that would be read past the last row, become 0
+// at any address; the bytes of a row's last ones behind `dim`, and those that would be read past the last row, become 0.  At most
+// PAD_GRID blocks, which go round: a thread for every 16 bytes of the largest call (64 GB and more of codes) would be a grid of 2^32.
+constexpr unsigned PAD_GRID = 1 << 18;
+
 __global__ __launch_bounds__(256) void pad_codes_kernel(const signed char* __restrict__ x, long long x_stride, int rows, int dim,
                                                         signed char* __restrict__ codes, int pitch) {
     const unsigned per = (unsigned)pitch / 16;
-    const unsigned long long id = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
-    const unsigned long long r = id / per;
-    if (r >= (unsigned long long)rows) return;
-    const int k = (int)(id - r * per) * 16, left = dim - k;          // left: bytes of the row from here
-    const signed char* from = x + (long long)r * x_stride;
-    i32x4 v = {0, 0, 0, 0};
-    if (left >= 16) {
-        __builtin_memcpy(&v, from + k, 16);
-    } else if (left > 0) {
-        unsigned long long lo = 0, hi = 0;
+    const unsigned long long all = (unsigned long long)rows * per;
+    for (unsigned long long id = (unsigned long long)blockIdx.x * 256 + threadIdx.x; id < all; id += (unsigned long long)gridDim.x * 256) {
+        const unsigned long long r = id / per;
+        const int k = (int)(id - r * per) * 16, left = dim - k;          // left: bytes of the row from here
+        const signed char* from = x + (long long)r * x_stride;
+        i32x4 v = {0, 0, 0, 0};
+        if (left >= 16) {
+            __builtin_memcpy(&v, from + k, 16);
+        } else if (left > 0) {
+            unsigned long long lo = 0, hi = 0;
 #pragma unroll
-        for (int i = 0; i < 15; ++i)
-            if (i < left) (i < 8 ? lo : hi) |= (unsigned long long)(unsigned char)from[k + i] << (8 * (i & 7));
-        v = i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+            for (int i = 0; i < 15; ++i)
+                if (i < left) (i < 8 ? lo : hi) |= (unsigned long long)(unsigned char)from[k + i] << (8 * (i & 7));
+            v = i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+        }
+        *(i32x4*)(codes + (long long)r * pitch + k) = v;
     }
-    *(i32x4*)(codes + (long long)r * pitch + k) = v;
 }
 
 // 16 bytes of a weight row; bytes at or past `dim` come as zeros and are not read
@@ -535,7 +539,7 @@ extern "C" int subreg_quantize_rows(const void* x, long long x_stride, int dtype
 
 static void pad_codes(const signed char* x, long long x_stride, int rows, int dim, signed char* codes, long long pitch, hipStream_t s) {
     const unsigned long long blocks = ((unsigned long long)rows * (pitch / 16) + 255) / 256;
-    hipLaunchKernelGGL(pad_codes_kernel, (unsigned)blocks, 256, 0, s, x, x_stride, rows, dim, codes, (int)pitch);
+    hipLaunchKernelGGL(pad_codes_kernel, blocks < PAD_GRID ? (unsigned)blocks : PAD_GRID, 256, 0, s, x, x_stride, rows, dim, codes, (int)pitch);
 }
 
 // the weight as the tile kernel reads it: rows at multiples of 16 bytes, 32-bit offsets inside a tile

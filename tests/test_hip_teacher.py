@@ -327,6 +327,20 @@ def test_linear_int8_steady_state_is_exact(m, k, n):
 
 
 @gpu
+def test_linear_int8_codes_past_one_pass_of_the_grid():
+    """More than 2^30 bytes of codes (2^26 threads' worth): rows at both ends and at the grid's turn are those of a call on them alone."""
+    m, k, n = 8500, 131071, 3
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
+    w = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    one = torch.ones(m, device="cuda")
+    got = HF.linear_int8(x, w, one[:n], None, one)
+    for rows in (slice(0, 40), slice(8180, 8220), slice(m - 40, m)):
+        want = x[rows].double() @ w.double().t().contiguous()
+        assert torch.equal(got[rows], want.float())
+
+
+@gpu
 def test_linear_int8_strides_and_leading_dimensions():
     x, wf = rnd((4, 6, 200), 1), rnd((90, 200), 2)
     w, ws = HF.quantize_rows(wf)
