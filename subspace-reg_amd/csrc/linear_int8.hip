@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * W, 2) void linear_int8_rows_kernel(
 // in flight are slower (250), and so is any other place of the DMAs in the stage (228 - 240).
 // D = C + A B with C and D the same accumulator registers.  As an asm statement because hipcc (ROCm 7.2) gives the builtin's result
 // other registers than its addend and copies between them (376 copies beside the 128 MFMAs of a stage).  The operands come from LDS reads
-// (the compiler waits for those before the statement); before the results are read, mfma_done() lets the last one retire.
+// (the compiler waits for those before the statement); before the results are read, settle_acc() below lets the last one retire.
 __device__ __forceinline__ void mfma_acc(i32x4& c, const i32x4& a, const i32x4& b) {
     asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }

@@ -207,21 +207,18 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 8) void top_logits_kernel(cons
     __syncthreads();
     unsigned t = 0;
     if (2 * top > min(loads, NT)) {
-        // few threads hold anything (at most two loads each: NT >= 2 top): their maxima say little, the border is sought among all logits
-        V x[2];
-        unsigned key[2 * N];
+        // few threads hold anything (one load each: NT >= 2 top, so loads < NT): their maxima say little, the border is sought among all logits
+        V x;
+        unsigned key[N];
+        const int skip = V::skip(tid, vocab);
+        x.load(row, V::at(tid, vocab));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = i * NT + tid, skip = V::skip(c, vocab);
-            x[i].load(row, V::at(c, vocab));
-#pragma unroll
-            for (int e = 0; e < N; ++e) key[i * N + e] = e >= skip ? TopKey<T>::of(x[i].elem(e)) : 0;
-        }
+        for (int e = 0; e < N; ++e) key[e] = e >= skip ? TopKey<T>::of(x.elem(e)) : 0;
         for (int b = TopKey<T>::BITS - 1; b >= 0; --b) {
             const unsigned want = t | (1u << b);
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < 2 * N; ++i) n += key[i] >= want;
+            for (int i = 0; i < N; ++i) n += key[i] >= want;
             n = block_reduce(n, red, 0, [](int a, int c) { return a + c; });
             if (n >= top) {
                 t = want;
