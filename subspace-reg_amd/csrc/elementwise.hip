@@ -628,7 +628,7 @@ extern "C" int subreg_dropblock_mask(const unsigned char* sample, unsigned char*
     SUBREG_CHECK_ARG(sample && keep_nhwc && kept_count && B > 0 && C > 0 && block_size >= 1 && H >= block_size && W >= block_size);
     hipStream_t s = (hipStream_t)stream;
     const size_t n = (size_t)B * C * H * W;
-    hipLaunchKernelGGL(keep_all_kernel, ew_blocks(n, 16), EW_THREADS, 0, s, keep_nhwc, n, kept_count);   // (no memset: a captured one is unsafe to replay)
+    hipLaunchKernelGGL(keep_all_kernel, ew_blocks(n, 16), EW_THREADS, 0, s, keep_nhwc, n, kept_count);   // (kernels, not memsets, in what a graph may record)
     hipLaunchKernelGGL(dropblock_mask_kernel, 1, 1024, 0, s, sample, keep_nhwc, B, C, H, W, block_size);
     size_t blocks = (n + 256 * 64 - 1) / (256 * 64);
     if (blocks > 2048) blocks = 2048;

@@ -440,11 +440,11 @@ class HipBackbone:
         """n streams whose kernels really run beside each other's and beside the current stream's.  HIP deals streams onto a few hardware
         queues in creation order, and two streams on one queue execute one after the other: in a process that had made
         other streams before, the two prefetch streams shared a queue and depth 2 ran like depth 1 (11.0 instead of 7.9 ms per nine
-        forwards, profiles/r06_prefetch_queues.txt: which stream counts collide depends on the priority, none is safe).  So the
+        forwards, profiles/r06_prefetch_queues.txt, recorded with two priorities: no stream count is safe).  So the
         streams are CHOSEN by measurement, once: a spin kernel on two candidates at a time - those that finish together in one
         spin's time run in parallel."""
         dev, cur = self.device, torch.cuda.current_stream()
-        cands = [torch.cuda.Stream(device=dev) for _ in range(10)]       # (all at the default priority: mixed priorities have hung here)
+        cands = [torch.cuda.Stream(device=dev) for _ in range(10)]       # (the default priority, as all streams here: a precaution)
         if os.environ.get("SUBREG_PREFETCH_CALIBRATE", "1") == "0":
             return cands[:n]
         spin = 2_000_000                                               # ticks of torch.cuda._sleep (~1 ms); only ratios are used

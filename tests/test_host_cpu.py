@@ -325,3 +325,17 @@ def test_episode_sampler_matches_reference_dataset_classes():
             seen |= cls
     with pytest.raises(ValueError):
         ep.BaseSplit(labels, 1, "nope")
+
+
+def test_every_stream_has_the_default_priority():
+    """Streams of one priority only, in the library, its tools, tests and the benchmark."""
+    own = os.path.abspath(__file__)
+    files = [os.path.join(d, f) for top in ("subspace-reg_amd", "tools", "tests", "perf", "oracle") for d, _, fs in os.walk(os.path.join(REPO, top))
+             for f in fs if f.endswith((".py", ".hip", ".h", ".cpp"))] + [os.path.join(REPO, f) for f in os.listdir(REPO) if f.endswith(".py")]
+    assert len(files) > 40
+    for path in files:
+        if os.path.abspath(path) == own:
+            continue
+        with open(path) as f:
+            found = re.search(r"Stream\([^)]*priority|StreamCreateWithPriority|is_high_priority_stream", f.read())
+        assert not found, (path, found and found.group(0))

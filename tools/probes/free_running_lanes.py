@@ -26,7 +26,7 @@ def main():
     params = {k: torch.from_numpy(np.array(v)).cuda() for k, v in sd.items() if v.dtype != np.int64}
     hb = HipBackbone(params, (1, 1, 2, 2), "bf16")
     N = 24
-    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream(priority=-1)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     print("%6s %12s %12s %12s %12s   (ms per forward of B images; joined = what ships)" % ("B", "joined", "free", "free+0.5", "one lane"))
     for B in batches:
         x = torch.randn(B, 3, 84, 84, device="cuda")

@@ -25,7 +25,7 @@ def main():
     ntn = Cout // 160
     w = (torch.randn(Cout, k * k, Cin, device=dev) / (Cin * k * k) ** 0.5).to(td)
     shift = torch.randn(Cout, device=dev)
-    s_main, s_side = torch.cuda.Stream(), torch.cuda.Stream(priority=-1)
+    s_main, s_side = torch.cuda.Stream(), torch.cuda.Stream()
     W256, W128, AUTO = _lib.CONV_KERNEL_WIDE | _lib.CONV_KERNEL_WIDE_256, _lib.CONV_KERNEL_WIDE | _lib.CONV_KERNEL_WIDE_128, 0
 
     def conv(x, y, B, flags, stream):
