@@ -971,3 +971,20 @@ def test_pretraining_with_a_teacher(int8_head):
     small = create_model("resnet12", 10, opt).cuda()
     with pytest.raises(ValueError):
         pretrain.train(1, [], small, None, optimizer, opt, teacher=teacher)
+
+
+@gpu
+def test_documented_lines_run():
+    """The lines on the operators in INTEGRATION.md, with an ordinary nn.Linear whose parameters want gradients."""
+    import os
+    import re
+
+    from conftest import REPO
+    with open(os.path.join(REPO, "INTEGRATION.md")) as f:
+        (block,) = [b for b in re.findall(r"```python\n(.*?)```", f.read(), re.S) if "HF.quantize_rows" in b]
+    names = dict(torch=torch, head=torch.nn.Linear(640, 351).cuda(), features=rnd((16, 640), 1), student_logits=rnd((16, 351), 2).requires_grad_(),
+                 target=torch.arange(16).cuda())
+    exec(block, names)                                               # (our own text)
+    _, want = plain_distill(names["student_logits"], names["values"], names["indices"], names["target"], 2.0, 1.0, 0.5)
+    _, elem = distill_bounds(names["student_logits"], names["values"], names["indices"], 2.0, 1.0, 0.5)
+    close(names["student_logits"].grad, want, elem)
