@@ -26,7 +26,7 @@ __device__ __forceinline__ float row_inverse(unsigned top, float* scale) {
 __device__ __forceinline__ int code_of(float x, float inv) { return __float2int_rn(x * inv); }
 
 // NT threads (a wave or a block of 256) per row, the row in registers: one read of x, 16 bytes a load, codes of a load in one store
-// (loads that overlap at the row's end write the same codes twice).  Bound by memory: 8192 x 4096 bf16 in 17.7 us, 5.7 TB/s (most of x
+// (loads that overlap at the row's end write the same codes twice).  Bound by memory: 8192 x 4096 bf16 in 17 us, 5.9 TB/s (most of x
 // comes from the last-level cache when it was just written).
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, long long x_stride, int rows, int dim,
@@ -207,7 +207,9 @@ __global__ __launch_bounds__(256, 4) void linear_int8_gemv_kernel(const signed c
 // Blocks and K: 16 NT channels a block so that there are 256 blocks or more, four waves, eight where K is cut for 64 channels (4096 long, us
 // with the quantiser, NT = 1 | 2 | 4: 64 x 4096 16.4 | 19.5 | 25.9; 64 x 8192 26.8 | 19.9 | 27.4; 48 x 16384 - | 28.9 | 27.0).  More than
 // one chunk in flight behind the current one is slower (48 x 16384: 31): the registers cost waves.
-// 48 x 4096 x 16384 moves its 67 MB in 21 us, 3.2 TB/s, and 16 rows in 16 us: the codes of x, read again by every block, are the rest.
+// 48 x 4096 x 16384 moves its 67 MB in 20 us, 3.3 TB/s, and 16 rows in 16 us: the codes of x, read again by every block, or the one chunk in
+// flight are the rest.  K % 128 != 0 costs more than its bytes: 48 x 2880 x 32768 52 us, K = 2944 41; 64 rows 63 and 47 - the last chunk is read byte
+// by byte, and in the instances with MT = 3, 4 and NT = 4, W = 8 spills 43 and 110 registers.
 constexpr int ROWS_MOST = 64, ROWS_GRID = 1024;
 
 template <typename T, int MT, int NT, int W>
@@ -318,10 +320,10 @@ __global__ __launch_bounds__(64 * W, 2) void linear_int8_rows_kernel(
 // Schedule of a stage (two k-steps): the reads of the second k-step run under the MFMAs of the first; the barrier stands in the MIDDLE
 // of the second k-step's MFMAs, and behind it the DMA of the stage after next and the reads of the next stage's first k-step run under
 // the other half.  A DMA has a whole stage of MFMAs to land.
-// 8192 x 4096 x 8192 takes 227 us (2.4 P operations a second; a large library product of 8-bit integers: 2.2).  What bounds it: the same
+// 8192 x 4096 x 8192 takes 229 - 238 us (2.3 P operations a second; a large library product of 8-bit integers: 2.2).  What bounds it: the same
 // kernel without the DMA takes 186, without the fragment reads 214, without both and the barrier 169, of which 145 are the MFMAs - at 1.8
 // GHz, where the clock is 2.0 with everything on and 2.4 at rest: the costs add up, as power does.  Four stages of 64 bytes with three
-// in flight are slower (250), and so is any other place of the DMAs in the stage (228 - 240).
+// in flight are slower (a whole call 267 against 245), and other places of the DMAs in the stage make no difference.
 // D = C + A B with C and D the same accumulator registers.  As an asm statement because hipcc (ROCm 7.2) gives the builtin's result
 // other registers than its addend and copies between them (376 copies beside the 128 MFMAs of a stage).  The operands come from LDS reads
 // (the compiler waits for those before the statement); before the results are read, settle_acc() below lets the last one retire.
