@@ -222,7 +222,7 @@ int subreg_conv_wgrad(const void* x, const void* dy, float* gw_packed, void* pad
 /* The same without float atomics in bf16: 1x1 convolutions (and the first layer's K=32 form), whose K splits subreg_conv_wgrad adds into
  * ONE copy in whatever order they end, store a copy each, so that a training step gives the same gradients bit for bit on every run.
  * gw_packed: subreg_conv_wgrad_ordered_splits(...) copies, all written; unpack with that number.  What a 3x3 convolution does is the
- * same in both forms.  f32 keeps its atomics (one copy). */
+ * same in both forms: copies on maps of up to 157 columns, atomics on wider ones.  f32 keeps its atomics (one copy). */
 int subreg_conv_wgrad_ordered_splits(int B, int H, int W, int Cin, int Cout, int ksize, int dtype);
 int subreg_conv_wgrad_ordered(const void* x, const void* dy, float* gw_packed, void* pad_x, void* pad_dy, int B, int H, int W, int Cin,
                               int Cout, int ksize, int dtype, void* stream);

@@ -988,3 +988,41 @@ def test_documented_lines_run():
     _, want = plain_distill(names["student_logits"], names["values"], names["indices"], names["target"], 2.0, 1.0, 0.5)
     _, elem = distill_bounds(names["student_logits"], names["values"], names["indices"], 2.0, 1.0, 0.5)
     close(names["student_logits"].grad, want, elem)
+
+
+@gpu
+def test_a_teacher_with_two_ranks_uneven_shards():
+    """train(..., teacher=, world=2): each rank's gradient carries n_local / n_global, an upstream factor other than 1, so that the sum
+    over ranks is the global mean's.  (Both ranks run here one after the other; what they exchange is tests/test_multirank.py's.)"""
+    from types import SimpleNamespace
+
+    from subreg_hip import pretrain, synthetic as syn
+    from subreg_hip.resnet_language import create_model
+
+    opt = SimpleNamespace(linear_bias=True, hip_dtype="f32", no_dropblock=True, print_freq=100, distill_temperature=2.0)
+    torch.manual_seed(0)
+    net, old = create_model("resnet12", 20, opt).cuda(), create_model("resnet12", 20, opt).cuda()
+    teacher = pretrain.Teacher(old, top=6)
+    x, y = torch.from_numpy(syn.make_images(3, 5, 32)), torch.tensor([0, 5, 7, 19, 2])
+    outs, grads = [], []
+    net.register_forward_hook(lambda m, i, o: outs.append(o.detach()))
+
+    class Watch:
+        param_groups = [dict(params=[])]
+
+        def zero_grad(self):
+            for p in net.parameters():
+                p.grad = None
+
+        def step(self):
+            grads.append(net.classifier.bias.grad.clone())
+
+    for rank, cut in ((0, slice(0, 3)), (1, slice(3, 5))):
+        pretrain.train(1, [(x, y)], net, None, Watch(), opt, rank=rank, world=2, log=lambda *a: None, teacher=teacher)
+        values, indices = teacher(x[cut].cuda())
+        out, share = outs[-1], outs[-1].shape[0] / 5
+        assert out.shape == (cut.stop - cut.start, 20)
+        _, want = plain_distill(out, values, indices, y[cut], 2.0, 0.5, 0.5)
+        _, elem = distill_bounds(out, values, indices, 2.0, 0.5, 0.5)
+        # three rows at most: their gradients' errors and the additions
+        close(grads[-1], share * want.sum(0), share * (3 * elem + 3 * U * want.abs().sum(0)))
