@@ -614,7 +614,8 @@ extern "C" int subreg_distill_loss(const subreg_distill_desc* d, void* stream) {
     SUBREG_CHECK_ARG(d->rows > 0 && d->rows <= MAX_ROWS && d->vocab > 0 && d->vocab <= MAX_COLUMNS && d->top >= 1 && d->top <= SUBREG_TOP_MAX);
     SUBREG_CHECK_ARG(d->logits_stride >= 0 && d->values_stride >= 0 && d->indices_stride >= 0 && d->grad_scale_stride >= 0);
     SUBREG_CHECK_ARG(float_dtype(d->dtype) && float_dtype(d->values_dtype) && d->temperature >= 1e-30f && d->temperature <= 1e15f);
-    SUBREG_CHECK_ARG(fabs((double)d->kd_weight) * d->temperature * fmax(d->temperature, 1.0) <= 1e30 && fabs((double)d->ce_weight) <= 1e30);
+    constexpr double MOST = 1e30 * (1.0 + 0x1p-20);   // (of numbers rounded to fp32)
+    SUBREG_CHECK_ARG(fabs((double)d->kd_weight) * d->temperature * fmax(d->temperature, 1.0) <= MOST && fabs((double)d->ce_weight) <= MOST);
     SUBREG_CHECK_ARG(d->reduction >= SUBREG_NONE && d->reduction <= SUBREG_MEAN);
     SUBREG_CHECK_ARG(!(d->flags & SUBREG_DISTILL_SKIP_UNIT) || (d->grad_scale && d->dlogits && !d->loss));
     SUBREG_CHECK_ARG(d->ws && ((size_t)d->ws & 255) == 0 && d->ws_bytes >= subreg_distill_ws_bytes(d->rows));

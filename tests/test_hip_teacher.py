@@ -693,6 +693,15 @@ def test_distill_kept_entries_and_labels_at_the_lowest_number(v, temp, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("temp,kd,ce", [(1.0, 1e30, 0.0), (1.0, 0.0, 1e30), (1e15, 1.0, 0.0), (1e-30, 1e30, 1e30), (1e10, -1e10, 0.0)])
+def test_distill_largest_weights(temp, kd, ce):
+    """The ends of what the arguments' check accepts are accepted below it, too (1e30 is a little more than 1e30 in fp32)."""
+    z, tv, ti, y = make_distill(4, 60, 4, torch.float32, 5)
+    for reduction in ("none", "mean"):
+        check_distill(z, tv, ti, y, temp, kd, ce, reduction)
+
+
+@gpu
 @pytest.mark.parametrize("v", [60, 3000, 140003])
 @pytest.mark.parametrize("reduction", [_lib.REDUCE_SUM, _lib.REDUCE_MEAN])
 def test_distill_counted_workspace(v, reduction):
